@@ -19,6 +19,8 @@ STATUS_NAMES = {0: "OK", 1: "INVALID_SIZE", 2: "INVALID_BATCH", 3: "MISALIGNED",
                 5: "TIMEOUT", 6: "PEER_UNAVAILABLE", 7: "INVALID_ARG", 8: "UNSUPPORTED"}
 MID_NONE, MID_MULTIPLY, MID_CONJ_MULTIPLY = 0, 1, 2
 LAYOUT_R8, LAYOUT_R8_BPERM, LAYOUT_R16, LAYOUT_R16_BPERM, LAYOUT_NATURAL = 0, 1, 2, 3, 4
+DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
+CACHE_MX4, CACHE_MX8 = 0, 1
 
 # every symbol the header declares, with its C signature
 _P, _I, _I64, _U32 = ct.c_void_p, ct.c_int, ct.c_int64, ct.c_uint32
@@ -64,7 +66,23 @@ SIGNATURES = {
     "fufft_peer_free": (_I, [_P]),
     "fufft_conv_multi_gpu": (_I, [_P]),
     "fufft_mg_chain": (_I, [_I64, _I, ct.POINTER(_I)]),
+    "fufft_mx4_codes_bytes": (ct.c_size_t, [_I64, _I64]),
+    "fufft_mx4_scales_bytes": (ct.c_size_t, [_I64, _I64]),
+    "fufft_mx4_quantize": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _P, _P, _P]),
+    "fufft_mx4_dequantize": (_I, [_P, _P, _I64, _I64, _P, _I, _I64, _P]),
+    "fufft_mx4_matmul": (_I, [_P, _P, _P, _P, _P, _P, _I, _I64, _I64, _I64, _I64, _P]),
+    "fufft_cache_append": (_I, [_P, _P, _I, _I64, _P, _P, _I64, _P]),
+    "fufft_cache_read": (_I, [_P, _P, _I, _I64, _P, _P, _I64, _P]),
+    "fufft_cache_read_channels": (_I, [_P, _P, _I, _I64, _P, _P, _P]),
+    "fufft_cache_conv_workspace": (ct.c_size_t, [_P, _I64]),
+    "fufft_cache_conv": (_I, [_P, _P, _P, _I, _I64, _I, _I64, _P, _I64, _P, _I, _I64, _P, ct.c_size_t, _P]),
 }
+
+
+class CacheDesc(ct.Structure):
+    """struct fufft_cache"""
+    _fields_ = [("codes", _P), ("scales", _P), ("page_table", _P), ("table_stride", _I64), ("kind", _I),
+                ("channels", _I), ("page_size", _I), ("pages", _I), ("max_pages", _I), ("batch", _I)]
 
 
 class FufftError(RuntimeError):

@@ -17,6 +17,13 @@ stream.  Names follow the reference:
 Complex data: torch.complex64 (or float32 with a trailing dim of 2), one
 transform per row of n points.  int16 BFP data: torch.int16 with a trailing
 dim of 2 (re, im) plus one float32 scale per transform.
+
+Operators without a counterpart there, for the layers around a long
+convolution of a sequence model: 4-bit microscaled matrices (Mx4,
+mx4_quantize, mx4_quantize_both, mx4_dequantize, mx4_matmul, mx4_linear,
+mx4_linear_grad) and the quantised sequence cache (SeqCache, cache_append,
+cache_read, cache_read_channels, cache_conv).  They take float32, float16 and
+bfloat16.
 """
 from __future__ import annotations
 
@@ -24,8 +31,9 @@ import ctypes as ct
 
 import torch
 
-from ._lib import (LAYOUT_NATURAL, LAYOUT_R8, LAYOUT_R8_BPERM, LAYOUT_R16, LAYOUT_R16_BPERM,
-                   MID_CONJ_MULTIPLY, MID_MULTIPLY, MID_NONE, FufftError, check, lib)
+from ._lib import (CACHE_MX4, CACHE_MX8, DTYPE_BF16, DTYPE_F16, DTYPE_F32, LAYOUT_NATURAL, LAYOUT_R8,
+                   LAYOUT_R8_BPERM, LAYOUT_R16, LAYOUT_R16_BPERM, MID_CONJ_MULTIPLY, MID_MULTIPLY, MID_NONE,
+                   CacheDesc, FufftError, check, lib)
 
 __all__ = [
     "MID_NONE", "MID_MULTIPLY", "MID_CONJ_MULTIPLY",
@@ -35,6 +43,8 @@ __all__ = [
     "conv_r2", "bfp_pack", "bfp_unpack", "conv_bfp", "pipeline_ip", "pipeline_fused", "pipeline_v16",
     "pipeline_v16f", "pipeline_r16", "pipeline_fwd", "pipeline_apply", "pipeline_v16_bfp", "init",
     "device_status", "launch_count", "max_n", "large_plan", "conv_large", "conv_large_bfp",
+    "Mx4", "mx4_empty", "mx4_quantize", "mx4_quantize_both", "mx4_dequantize", "mx4_matmul", "mx4_linear",
+    "mx4_linear_grad", "SeqCache", "seq_cache", "cache_append", "cache_read", "cache_read_channels", "cache_conv",
 ]
 
 
@@ -400,3 +410,257 @@ def pipeline_apply(spec, b_dr, n, mid=MID_MULTIPLY):
 def pipeline_v16_bfp(aq, a_scale, bq, b_scale, n):
     """fufft_pipeline_v16_bfp: int16 BFP in and out, radix-16 chain"""
     return conv_bfp(aq, a_scale, bq, b_scale, n, LAYOUT_R16, MID_MULTIPLY)
+
+
+# ---- microscaled 4-bit matrices -------------------------------------------------------
+_DTYPES = {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}
+
+
+def _dtype(t: torch.dtype) -> int:
+    d = _DTYPES.get(t)
+    if d is None:
+        raise TypeError(f"expected float32, float16 or bfloat16, got {t}")
+    return d
+
+
+def _rows(t: torch.Tensor, what: str) -> torch.Tensor:
+    """a CUDA tensor of rows: unit stride along the last dimension"""
+    if not t.is_cuda:
+        raise ValueError("fufft_b200 operates on CUDA tensors")
+    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1) or (t.stride(0) < t.shape[1] and t.shape[0] > 1):
+        raise ValueError(f"{what} must be a 2-D tensor with unit stride along its rows")
+    return t
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _i32(t: torch.Tensor, n: int, what: str):
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n:
+        raise ValueError(f"{what} must be int32 with {n} entries")
+    return _ptr(t)
+
+
+class Mx4:
+    """A [rows, cols] matrix in 4-bit microscaled blocks along its columns:
+    codes uint8 [rows, ceil(cols / 256) * 128] and the tiled E8M0 scales uint8
+    [ceil(rows / 128), ceil(cols / 256) * 2, 32, 4, 4] (layout in
+    include/fufft_b200.h, fufft_mx4_*)"""
+    __slots__ = ("codes", "scales", "rows", "cols")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, cols: int):
+        tiles = -(-cols // 256) * 2
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+            raise TypeError("codes and scales must be uint8")
+        if codes.numel() != rows * tiles * 64 or scales.numel() != -(-rows // 128) * tiles * 512:
+            raise ValueError(f"codes or scales do not fit a {rows} x {cols} matrix")
+        self.codes, self.scales, self.rows, self.cols = codes, scales, rows, cols
+
+    @property
+    def shape(self) -> tuple[int, int]:
+        return self.rows, self.cols
+
+
+def mx4_empty(rows: int, cols: int, device=None) -> Mx4:
+    """uninitialised buffers of a 4-bit matrix"""
+    tiles = -(-cols // 256) * 2
+    return Mx4(torch.empty(rows, tiles * 64, dtype=torch.uint8, device=device or "cuda"),
+               torch.empty(-(-rows // 128), tiles, 32, 4, 4, dtype=torch.uint8, device=device or "cuda"), rows, cols)
+
+
+def _quantize(x: torch.Tensor, q: Mx4 | None, qt: Mx4 | None) -> None:
+    check(lib().fufft_mx4_quantize(x.data_ptr(), _dtype(x.dtype), x.shape[0], x.shape[1], _row_stride(x),
+                                   None if q is None else _ptr(q.codes), None if q is None else _ptr(q.scales),
+                                   None if qt is None else _ptr(qt.codes), None if qt is None else _ptr(qt.scales),
+                                   _stream()), "fufft_mx4_quantize")
+
+
+def _turned(x: torch.Tensor) -> bool:
+    """a transposed view: quantised along the other axis of what it is a view of"""
+    return x.is_cuda and x.dim() == 2 and x.stride(0) == 1 and x.stride(1) != 1 and x.shape[0] > 1
+
+
+def mx4_quantize(x: torch.Tensor, transpose: bool = False) -> Mx4:
+    """x [rows, cols] quantised in blocks of 32 along its rows, or, with
+    `transpose`, x^T quantised along the columns of x"""
+    if _turned(x):
+        x, transpose = x.t(), not transpose
+    x = _rows(x, "x")
+    rows, cols = x.shape
+    if transpose:
+        q = mx4_empty(cols, rows, x.device)
+        _quantize(x, None, q)
+    else:
+        q = mx4_empty(rows, cols, x.device)
+        _quantize(x, q, None)
+    return q
+
+
+def mx4_quantize_both(x: torch.Tensor) -> tuple[Mx4, Mx4]:
+    """(mx4_quantize(x), mx4_quantize(x, transpose=True)) from one read of x"""
+    if _turned(x):
+        return mx4_quantize_both(x.t())[::-1]
+    x = _rows(x, "x")
+    q, qt = mx4_empty(x.shape[0], x.shape[1], x.device), mx4_empty(x.shape[1], x.shape[0], x.device)
+    _quantize(x, q, qt)
+    return q, qt
+
+
+def mx4_dequantize(q: Mx4, dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None) -> torch.Tensor:
+    """the values that q stands for"""
+    if out is None:
+        out = torch.empty(q.rows, q.cols, dtype=dtype, device=q.codes.device)
+    elif out.dtype != dtype or out.shape != q.shape:
+        raise ValueError(f"out must be {dtype} {q.shape}")
+    check(lib().fufft_mx4_dequantize(_ptr(q.codes), _ptr(q.scales), q.rows, q.cols, _rows(out, "out").data_ptr(),
+                                     _dtype(dtype), _row_stride(out), _stream()), "fufft_mx4_dequantize")
+    return out
+
+
+def mx4_matmul(a: Mx4, b: Mx4, dtype: torch.dtype = torch.bfloat16, bias: torch.Tensor | None = None,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """a b^T + bias: [a.rows, b.rows] in `dtype`, summed in float32; both are
+    blocked along the summed axis, bias is float32 [b.rows]"""
+    if a.cols != b.cols:
+        raise ValueError(f"the summed axes differ: {a.shape} and {b.shape}")
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (b.rows,)):
+        raise ValueError(f"bias must be float32 with {b.rows} entries")
+    if out is None:
+        out = torch.empty(a.rows, b.rows, dtype=dtype, device=a.codes.device)
+    elif out.dtype != dtype or out.shape != (a.rows, b.rows):
+        raise ValueError(f"out must be {dtype} {(a.rows, b.rows)}")
+    check(lib().fufft_mx4_matmul(_ptr(a.codes), _ptr(a.scales), _ptr(b.codes), _ptr(b.scales), _ptr(bias),
+                                 _rows(out, "out").data_ptr(), _dtype(dtype), a.rows, b.rows, a.cols,
+                                 _row_stride(out), _stream()), "fufft_mx4_matmul")
+    return out
+
+
+def mx4_linear(x: torch.Tensor, w: Mx4, bias: torch.Tensor | None = None,
+               dtype: torch.dtype | None = None) -> torch.Tensor:
+    """x [..., k] quantised along k, times w [n, k]: [..., n] in x's dtype unless another is given"""
+    y = mx4_matmul(mx4_quantize(x.reshape(-1, x.shape[-1])), w, dtype or x.dtype, bias)
+    return y.view(*x.shape[:-1], w.rows)
+
+
+def mx4_linear_grad(gy: torch.Tensor, xt: Mx4, wt: Mx4,
+                    dtype: torch.dtype | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """gradients of y = x w^T [m, n] with every operand in 4 bits, the
+    quantiser passed straight through: gx [m, k] = Q(gy) Q(w^T)^T and
+    gw [n, k] = Q(gy^T) Q(x^T)^T, from xt = mx4_quantize(x, transpose=True)
+    [k, m] and wt = mx4_quantize(w, transpose=True) [k, n]"""
+    if gy.dim() != 2 or xt.cols != gy.shape[0] or wt.cols != gy.shape[1] or xt.rows != wt.rows:
+        raise ValueError(f"gy {tuple(gy.shape)} does not fit xt {xt.shape} and wt {wt.shape}")
+    gq, gt = mx4_quantize_both(gy)
+    return mx4_matmul(gq, wt, dtype or gy.dtype), mx4_matmul(gt, xt, dtype or gy.dtype)
+
+
+# ---- quantised sequence cache -----------------------------------------------------------
+_KINDS = {"mx4": CACHE_MX4, "mx8": CACHE_MX8}
+
+
+class SeqCache:
+    """Past inputs of a batch of sequences in pages, each token's channels in
+    microscaled blocks of 32 (`kind` "mx4" or "mx8"):
+      codes       uint8 [pages, page_size, channels / 2 (mx4) or channels (mx8)]
+      scales      uint8 [pages, page_size, channels / 32]
+      page_table  int32 [batch, max_pages], -1 where there is no page"""
+    __slots__ = ("codes", "scales", "page_table", "kind", "channels", "desc", "_at")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, page_table: torch.Tensor, kind: str):
+        if kind not in _KINDS:
+            raise ValueError(f"kind must be one of {sorted(_KINDS)}")
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or page_table.dtype != torch.int32:
+            raise TypeError("codes and scales must be uint8, page_table int32")
+        if codes.dim() != 3 or scales.dim() != 3 or page_table.dim() != 2 or codes.shape[:2] != scales.shape[:2]:
+            raise ValueError("codes and scales must be [pages, page_size, ...], page_table [batch, max_pages]")
+        channels = scales.shape[2] * 32
+        if codes.shape[2] != (channels // 2 if kind == "mx4" else channels):
+            raise ValueError("codes and scales differ in their channels")
+        if not page_table.is_cuda or (page_table.stride(1) != 1 and page_table.shape[1] > 1):
+            raise ValueError("page_table must be a CUDA tensor with unit stride along its rows")
+        self.codes, self.scales, self.page_table, self.kind, self.channels = codes, scales, page_table, kind, channels
+        stride = page_table.stride(0) if page_table.shape[0] > 1 else page_table.shape[1]
+        self.desc = CacheDesc(_ptr(codes), _ptr(scales), page_table.data_ptr(), stride, _KINDS[kind], channels,
+                              codes.shape[1], codes.shape[0], page_table.shape[1], page_table.shape[0])
+        self._at = ct.addressof(self.desc)
+
+    @property
+    def batch(self) -> int:
+        return self.page_table.shape[0]
+
+
+def seq_cache(pages: int, page_size: int, channels: int, page_table: torch.Tensor, kind: str = "mx8") -> SeqCache:
+    """an empty cache on page_table's device"""
+    if channels % 32:
+        raise ValueError("channels must be a multiple of 32")
+    make = dict(dtype=torch.uint8, device=page_table.device)
+    return SeqCache(torch.zeros(pages, page_size, channels // 2 if kind == "mx4" else channels, **make),
+                    torch.zeros(pages, page_size, channels // 32, **make), page_table, kind)
+
+
+def cache_append(cache: SeqCache, x: torch.Tensor, cu: torch.Tensor, starts: torch.Tensor) -> None:
+    """quantise the tokens x [tokens, channels] into the cache: tokens
+    cu[b] .. cu[b + 1] - 1 go to sequence b from position starts[b] on"""
+    x = _rows(x, "x")
+    if x.shape[1] != cache.channels:
+        raise ValueError(f"x must have {cache.channels} channels")
+    check(lib().fufft_cache_append(cache._at, x.data_ptr(), _dtype(x.dtype), _row_stride(x),
+                                   _i32(cu, cache.batch + 1, "cu"), _i32(starts, cache.batch, "starts"), x.shape[0],
+                                   _stream()), "fufft_cache_append")
+
+
+def cache_read(cache: SeqCache, cu: torch.Tensor, starts: torch.Tensor, tokens: int,
+               dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None) -> torch.Tensor:
+    """stored values [tokens, channels] of the ragged run (cu, starts), as in cache_append"""
+    if out is None:
+        out = torch.empty(tokens, cache.channels, dtype=dtype, device=cache.codes.device)
+    elif out.dtype != dtype or out.shape != (tokens, cache.channels):
+        raise ValueError(f"out must be {dtype} {(tokens, cache.channels)}")
+    if cache.batch == 0:
+        out.zero_()
+    check(lib().fufft_cache_read(cache._at, _rows(out, "out").data_ptr(), _dtype(dtype), _row_stride(out),
+                                 _i32(cu, cache.batch + 1, "cu"), _i32(starts, cache.batch, "starts"), tokens,
+                                 _stream()), "fufft_cache_read")
+    return out
+
+
+def cache_read_channels(cache: SeqCache, starts: torch.Tensor, counts: torch.Tensor, n: int,
+                        dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """[batch, channels, n]: positions starts[b] .. starts[b] + counts[b] - 1 of
+    every sequence, channel by channel, zeros from counts[b] on -- two of
+    these rows are what conv_r2 takes"""
+    out = torch.empty(cache.batch, cache.channels, n, dtype=dtype, device=cache.codes.device)
+    check(lib().fufft_cache_read_channels(cache._at, out.data_ptr(), _dtype(dtype), n,
+                                          _i32(starts, cache.batch, "starts"), _i32(counts, cache.batch, "counts"),
+                                          _stream()), "fufft_cache_read_channels")
+    return out
+
+
+def cache_conv(cache: SeqCache, lengths: torch.Tensor, taps: torch.Tensor, gate: torch.Tensor | None = None,
+               dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None,
+               workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """newest output of a causal convolution per sequence, [batch, channels]:
+    gate[b, c] * sum_j taps[j, c // (channels // heads)] * x[b, lengths[b] - 1 - j, c]
+    over j < min(lengths[b], len(taps)); taps [n_taps, heads] float32 or
+    bfloat16, gate [batch, channels] of `dtype` or None"""
+    taps = _rows(taps, "taps")
+    if taps.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError("taps must be float32 or bfloat16")
+    if out is None:
+        out = torch.empty(cache.batch, cache.channels, dtype=dtype, device=cache.codes.device)
+    elif out.dtype != dtype or out.shape != (cache.batch, cache.channels):
+        raise ValueError(f"out must be {dtype} {(cache.batch, cache.channels)}")
+    if gate is not None and (gate.dtype != dtype or gate.shape != out.shape):
+        raise ValueError(f"gate must be {dtype} {tuple(out.shape)}")
+    if workspace is None:
+        need = lib().fufft_cache_conv_workspace(cache._at, taps.shape[0])
+        if need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=out.device)
+    check(lib().fufft_cache_conv(cache._at, _i32(lengths, cache.batch, "lengths"), taps.data_ptr(), _dtype(taps.dtype),
+                                 taps.shape[0], taps.shape[1], _row_stride(taps),
+                                 None if gate is None else _rows(gate, "gate").data_ptr(),
+                                 0 if gate is None else _row_stride(gate), _rows(out, "out").data_ptr(), _dtype(dtype),
+                                 _row_stride(out), _ptr(workspace), 0 if workspace is None else workspace.numel(),
+                                 _stream()), "fufft_cache_conv")
+    return out

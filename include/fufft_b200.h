@@ -396,6 +396,89 @@ fufft_status fufft_conv_large_bfp_noalloc(const int16_t* aq, const float* a_scal
                                           int64_t batch, int r_out, int mid, fufft_layout layout,
                                           fufft_midop mid_op, fufft_stream_t stream);
 
+/* ---- microscaled 4-bit matrices (no reference counterpart) ---------------
+ * A [rows][cols] matrix in blocks of 32 columns: 4-bit E2M1 elements (0 .5 1
+ * 1.5 2 3 4 6 and their negatives) under one power-of-two scale a block.
+ *   codes   [rows][pitch] bytes, pitch = ceil(cols / 256) * 128: two elements
+ *           a byte, the lower column in the low half; zero beyond cols.
+ *   scales  one byte s per block, the block's scale is 2^(s - 127) (E8M0;
+ *           255 = NaN).  Stored in tiles of 128 rows x 4 blocks of 512 bytes,
+ *           [ceil(rows / 128)][pitch / 64][32][4][4] = [row tile][block tile]
+ *           [row % 32][row / 32 % 4][block % 4]: what the tensor cores take.
+ *           Bytes of rows beyond `rows` are never used.
+ *   s - 127 = max(-127, floor(log2(max|x|)) - 2); elements are x / scale
+ *   rounded to nearest even, saturating at 6.  An infinity or a NaN makes its
+ *   whole block NaN.
+ * Both buffers are 16-byte aligned, fufft_mx4_codes_bytes / _scales_bytes long.
+ *
+ * quantize: x has unit column stride and `row_stride` elements between rows.
+ *   codes / scales get the blocks along the rows, codes_t / scales_t the
+ *   matrix transposed ([cols][rows], blocks along the columns of x); either
+ *   pair may be NULL, both come from one read of x.
+ * matmul: out[m][n] = sum_k a[m][k] b[n][k] + bias[n] (bias may be NULL),
+ *   a [m][k] and b [n][k] as above, summed in fp32 and rounded once to dtype.
+ *   A block scale of 255 gives NaN in the outputs that it enters. */
+typedef enum fufft_dtype { FUFFT_F32 = 0, FUFFT_F16 = 1, FUFFT_BF16 = 2 } fufft_dtype;
+size_t fufft_mx4_codes_bytes(int64_t rows, int64_t cols);
+size_t fufft_mx4_scales_bytes(int64_t rows, int64_t cols);
+fufft_status fufft_mx4_quantize(const void* x, fufft_dtype dtype, int64_t rows, int64_t cols, int64_t row_stride,
+                                uint8_t* codes, uint8_t* scales, uint8_t* codes_t, uint8_t* scales_t,
+                                fufft_stream_t stream);
+fufft_status fufft_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t cols, void* out,
+                                  fufft_dtype dtype, int64_t row_stride, fufft_stream_t stream);
+fufft_status fufft_mx4_matmul(const uint8_t* a_codes, const uint8_t* a_scales, const uint8_t* b_codes,
+                              const uint8_t* b_scales, const float* bias, void* out, fufft_dtype dtype, int64_t m,
+                              int64_t n, int64_t k, int64_t out_stride, fufft_stream_t stream);
+
+/* ---- quantised sequence cache (no reference counterpart) -----------------
+ * The past inputs of `batch` sequences in pages of page_size tokens, each
+ * token's channels (a multiple of 32) in blocks of 32 under one power-of-two
+ * scale: MX4 as above, or MX8 with E4M3 elements (s - 127 = max(-127,
+ * floor(log2(max|x|)) - 8), saturating at 448).
+ *   codes       [pages][page_size][channels / 2 (MX4) or channels (MX8)]
+ *   scales      [pages][page_size][channels / 32]
+ *   page_table  [batch][max_pages] int32, table_stride apart: page of tokens
+ *               k * page_size ... of a sequence; outside 0 .. pages - 1 (-1,
+ *               say) means that there is none.
+ * Sequences, positions and lengths are on the device; runs of tokens are
+ * ragged: token t belongs to sequence b with cu[b] <= t < cu[b + 1] (cu: int32
+ * [batch + 1], not decreasing) and stands at position starts[b] + t - cu[b].
+ *   append: quantises x[t][...] into its place.  Tokens without a page, or
+ *     outside cu, are dropped.  Two tokens of one call at one place race.
+ *   read: out[t][...] = the stored values; zeros without a page.
+ *   read_channels: out[b][c][i], i < n, = position starts[b] + i for
+ *     i < counts[b], zeros beyond: rows for fufft_conv_r2_f32 and its like.
+ *   conv: one output of a causal convolution per sequence, over its last
+ *     min(lengths[b], n_taps) tokens:
+ *       out[b][c] = gate[b][c] * sum_j taps[j][c / (channels / heads)]
+ *                                      * x[b][lengths[b] - 1 - j][c]
+ *     heads divides channels; taps fp32 or bf16 with taps_stride between lags;
+ *     gate (dtype of out, may be NULL); positions without a page count as
+ *     zeros, a length of zero gives zero.  Sums are fp32, in an order that
+ *     depends on the sizes alone.  workspace: fufft_cache_conv_workspace
+ *     bytes, 16-byte aligned, not used by anything else until the call's work
+ *     has finished. */
+typedef enum fufft_cache_kind { FUFFT_CACHE_MX4 = 0, FUFFT_CACHE_MX8 = 1 } fufft_cache_kind;
+typedef struct fufft_cache {
+   uint8_t* codes;
+   uint8_t* scales;
+   const int32_t* page_table;
+   int64_t table_stride;
+   fufft_cache_kind kind;
+   int channels, page_size, pages, max_pages, batch;
+} fufft_cache;
+fufft_status fufft_cache_append(const fufft_cache* cache, const void* x, fufft_dtype dtype, int64_t row_stride,
+                                const int32_t* cu, const int32_t* starts, int64_t tokens, fufft_stream_t stream);
+fufft_status fufft_cache_read(const fufft_cache* cache, void* out, fufft_dtype dtype, int64_t row_stride,
+                              const int32_t* cu, const int32_t* starts, int64_t tokens, fufft_stream_t stream);
+fufft_status fufft_cache_read_channels(const fufft_cache* cache, void* out, fufft_dtype dtype, int64_t n,
+                                       const int32_t* starts, const int32_t* counts, fufft_stream_t stream);
+size_t fufft_cache_conv_workspace(const fufft_cache* cache, int64_t n_taps);
+fufft_status fufft_cache_conv(const fufft_cache* cache, const int32_t* lengths, const void* taps,
+                              fufft_dtype taps_dtype, int64_t n_taps, int heads, int64_t taps_stride,
+                              const void* gate, int64_t gate_stride, void* out, fufft_dtype dtype,
+                              int64_t out_stride, void* workspace, size_t workspace_bytes, fufft_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
