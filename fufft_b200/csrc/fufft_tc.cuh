@@ -1,0 +1,106 @@
+// fufft_tc.cuh -- tensor-core building blocks for sm_100a (inline PTX):
+// tensor memory, block-scaled 4-bit products, their shared-memory and
+// instruction descriptors, and TMA tiles of 128-byte rows.
+#pragma once
+#include "fufft_device.cuh"
+
+namespace fufft {
+namespace tc {
+
+// ---- tensor memory ---------------------------------------------------------
+// COLS: a power of two, 32 .. 512; one whole warp allocates and frees
+template<int COLS> __device__ __forceinline__ void tmem_alloc(uint32_t* at_smem)
+{
+   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(at_smem)), "n"(COLS) : "memory");
+   asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+template<int COLS> __device__ __forceinline__ void tmem_free(uint32_t at)
+{
+   asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(at), "n"(COLS));
+}
+__device__ __forceinline__ void fence_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_load_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// 16 consecutive columns of the warp's 32 lanes
+__device__ __forceinline__ void tmem_load16(uint32_t at, float* v)
+{
+   uint32_t r[16];
+   asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+                "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                  "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                : "r"(at));
+#pragma unroll
+   for(int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// ---- descriptors -----------------------------------------------------------
+// rows of 128 bytes, the 16-byte chunks of a row permuted by TMA's 128-byte
+// swizzle, groups of eight rows 1024 bytes apart; `at` may step by 32 bytes
+// (64 4-bit values) inside the row
+__device__ __forceinline__ uint64_t rows_desc(uint32_t at)
+{
+   return (uint64_t)((at & 0x3ffff) >> 4) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+// 32 rows of 16 bytes, plain: what a 32x128b copy to tensor memory reads
+__device__ __forceinline__ uint64_t scales_desc(uint32_t at)
+{
+   return (uint64_t)((at & 0x3ffff) >> 4) | (8ull << 32) | (1ull << 46);
+}
+// kind::mxf4: both operands E2M1, scales E8M0, M x N outputs; `sf` = byte (0
+// or 2) of the 32-bit scale column that holds the two blocks of this step
+__host__ __device__ constexpr uint32_t mxf4_idesc(int m, int n, int sf)
+{
+   return (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 7) << 27) |
+          ((uint32_t)sf << 29) | ((uint32_t)sf << 4);
+}
+
+// one 512-byte scale tile (128 rows x 4 blocks) -> four columns of tensor
+// memory, the same in all four 32-lane quarters
+__device__ __forceinline__ void copy_scales(uint32_t to_tmem, uint64_t desc)
+{
+   asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" :: "r"(to_tmem), "l"(desc) : "memory");
+}
+// D[128 x N] (+)= A[128 x 64] B[N x 64]^T under their scales
+__device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                         bool add)
+{
+   asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %6, 0;\n\t"
+                "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+                :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"((uint32_t)add) : "memory");
+}
+// the barrier completes when all the tensor work issued so far by this thread has
+__device__ __forceinline__ void commit(uint64_t* bar)
+{
+   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(smem_u32(bar)) : "memory");
+}
+
+// ---- clusters --------------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_rank()
+{
+   uint32_t r;
+   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+   return r;
+}
+// all threads of all CTAs of the cluster; orders their shared-memory accesses
+__device__ __forceinline__ void cluster_sync()
+{
+   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// address in CTA `rank`'s shared memory of what `p` is in this one's
+__device__ __forceinline__ uint32_t peer_smem(const void* p, uint32_t rank)
+{
+   uint32_t r;
+   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+   return r;
+}
+__device__ __forceinline__ float load_peer(uint32_t at)
+{
+   float v;
+   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+   return v;
+}
+
+}  // namespace tc
+}  // namespace fufft
