@@ -148,6 +148,7 @@ fufft_status check_cache(const fufft_cache* c)
    if(c->channels <= 0 || c->channels % mx::BLOCK || c->channels > MAX_CHANNELS || c->page_size <= 0 || c->pages < 0 ||
       c->max_pages < 0)
       return FUFFT_ERR_INVALID_SIZE;
+   if((long long)c->pages * c->page_size > 0x7fffffffll) return FUFFT_ERR_INVALID_SIZE;   // a row index is 32 bits
    if(c->batch < 0 || c->batch > MAX_BATCH) return FUFFT_ERR_INVALID_BATCH;
    if(c->batch == 0) return FUFFT_OK;
    if(c->table_stride < c->max_pages) return FUFFT_ERR_INVALID_ARG;

@@ -20,9 +20,23 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
-#include "../../include/fufft_b200.h"
+#include "fufft_internal.cuh"
 
 namespace fufft {
+namespace host {
+// lets `kern` use `bytes` of dynamic shared memory on the current device, once per device (a bit of `done` each)
+template<class K> fufft_status allow_smem(K kern, int bytes, std::atomic<uint64_t>& done)
+{
+   int dev = 0;
+   fufft_status s = check(cudaGetDevice(&dev));
+   if(s != FUFFT_OK) return s;
+   const uint64_t bit = 1ull << (dev & 63);
+   if(done.load(std::memory_order_acquire) & bit) return FUFFT_OK;
+   s = check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+   if(s == FUFFT_OK) done.fetch_or(bit, std::memory_order_acq_rel);
+   return s;
+}
+}  // namespace host
 namespace mx {
 
 constexpr int BLOCK = 32;         // values per scale

@@ -228,7 +228,8 @@ fufft_status launch_split(const Operands& o, int split, const DeviceCtx& ctx, cu
       if((s = codes_tmap(&tq, o.a, o.m, pitch, BN)) != FUFFT_OK) return s;
    }
    auto kern = matmul_split_kernel<T, BN>;
-   if((s = check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM))) != FUFFT_OK) return s;
+   static std::atomic<uint64_t> configured{0};
+   if((s = allow_smem(kern, C::SMEM, configured)) != FUFFT_OK) return s;
    MatmulArgs g{o.b_scale, o.a_scale, o.bias, o.out, ctx.status, o.n, o.m, o.out_stride, (int)(pitch / 128),
                 (int)ceil_div(o.n, 128), split};
    cudaLaunchConfig_t cfg = {};

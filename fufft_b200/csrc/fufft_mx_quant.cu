@@ -133,7 +133,8 @@ fufft_status quantize(const void* x, long long rows, long long cols, long long r
       quantize_rows_kernel<T><<<(unsigned)ceil_div(warps, 8), 256, 0, st>>>(p, rows, cols, row_stride, codes, scales, vec);
    } else {
       constexpr int SMEM = QT * QT_PITCH * (int)sizeof(float);
-      fufft_status s = check(cudaFuncSetAttribute(quantize_tile_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+      static std::atomic<uint64_t> configured{0};
+      fufft_status s = allow_smem(quantize_tile_kernel<T>, SMEM, configured);
       if(s != FUFFT_OK) return s;
       const long long tiles = mx4_scale_tiles(rows) * mx4_scale_tiles(cols);
       quantize_tile_kernel<T><<<(unsigned)tiles, 256, SMEM, st>>>(p, rows, cols, row_stride, codes, scales, codes_t,
