@@ -71,6 +71,7 @@ SIGNATURES = {
     "fufft_mx4_quantize": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _P, _P, _P]),
     "fufft_mx4_dequantize": (_I, [_P, _P, _I64, _I64, _P, _I, _I64, _P]),
     "fufft_mx4_matmul": (_I, [_P, _P, _P, _P, _P, _P, _I, _I64, _I64, _I64, _I64, _P]),
+    "fufft_mx4_linear": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _P, _P, _I, _I64, _P]),
     "fufft_cache_append": (_I, [_P, _P, _I, _I64, _P, _P, _I64, _P]),
     "fufft_cache_read": (_I, [_P, _P, _I, _I64, _P, _P, _I64, _P]),
     "fufft_cache_read_channels": (_I, [_P, _P, _I, _I64, _P, _P, _P]),

@@ -272,11 +272,10 @@ template<class T> fufft_status matmul(const Operands& o, cudaStream_t st)
 }  // namespace mx
 }  // namespace fufft
 
-extern "C" {
-
-fufft_status fufft_mx4_matmul(const uint8_t* a_codes, const uint8_t* a_scales, const uint8_t* b_codes,
-                              const uint8_t* b_scales, const float* bias, void* out, fufft_dtype dtype, int64_t m,
-                              int64_t n, int64_t k, int64_t out_stride, fufft_stream_t stream)
+namespace {
+fufft_status check_matmul(const uint8_t* a_codes, const uint8_t* a_scales, const uint8_t* b_codes, const uint8_t* b_scales,
+                          const float* bias, const void* out, fufft_dtype dtype, int64_t m, int64_t n, int64_t k,
+                          int64_t out_stride)
 {
    constexpr int64_t MAX = 1ll << 30;
    if(dtype < FUFFT_F32 || dtype > FUFFT_BF16) return FUFFT_ERR_INVALID_ARG;
@@ -287,6 +286,18 @@ fufft_status fufft_mx4_matmul(const uint8_t* a_codes, const uint8_t* a_scales, c
    if(!aligned(a_codes, 16) || !aligned(a_scales, 16) || !aligned(b_codes, 16) || !aligned(b_scales, 16) ||
       !aligned(bias, 4) || !aligned(out, dtype == FUFFT_F32 ? 4 : 2))
       return FUFFT_ERR_MISALIGNED;
+   return FUFFT_OK;
+}
+}  // namespace
+
+extern "C" {
+
+fufft_status fufft_mx4_matmul(const uint8_t* a_codes, const uint8_t* a_scales, const uint8_t* b_codes,
+                              const uint8_t* b_scales, const float* bias, void* out, fufft_dtype dtype, int64_t m,
+                              int64_t n, int64_t k, int64_t out_stride, fufft_stream_t stream)
+{
+   fufft_status s = check_matmul(a_codes, a_scales, b_codes, b_scales, bias, out, dtype, m, n, k, out_stride);
+   if(s != FUFFT_OK || m == 0 || n == 0) return s;
    const mx::Operands o{a_codes, a_scales, b_codes, b_scales, bias, out, m, n, k, out_stride};
    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
    switch(dtype) {
@@ -294,6 +305,18 @@ fufft_status fufft_mx4_matmul(const uint8_t* a_codes, const uint8_t* a_scales, c
    case FUFFT_F16: return mx::matmul<__half>(o, st);
    default: return mx::matmul<__nv_bfloat16>(o, st);
    }
+}
+
+fufft_status fufft_mx4_linear(const void* x, fufft_dtype x_dtype, int64_t m, int64_t k, int64_t x_stride,
+                              uint8_t* x_codes, uint8_t* x_scales, const uint8_t* w_codes, const uint8_t* w_scales,
+                              int64_t n, const float* bias, void* out, fufft_dtype dtype, int64_t out_stride,
+                              fufft_stream_t stream)
+{
+   // everything is checked before the first launch: a refused call leaves x_codes alone
+   fufft_status s = check_matmul(x_codes, x_scales, w_codes, w_scales, bias, out, dtype, m, n, k, out_stride);
+   if(s != FUFFT_OK || m == 0 || n == 0) return s;
+   if((s = fufft_mx4_quantize(x, x_dtype, m, k, x_stride, x_codes, x_scales, nullptr, nullptr, stream)) != FUFFT_OK) return s;
+   return fufft_mx4_matmul(x_codes, x_scales, w_codes, w_scales, bias, out, dtype, m, n, k, out_stride, stream);
 }
 
 }  // extern "C"

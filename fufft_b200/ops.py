@@ -413,7 +413,15 @@ def pipeline_v16_bfp(aq, a_scale, bq, b_scale, n):
 
 
 # ---- microscaled 4-bit matrices -------------------------------------------------------
+# These operators run at a few microseconds, the time of their own Python: one
+# allocation for the two buffers of a matrix, no check made twice.
 _DTYPES = {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}
+_raw_stream, _device_index = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+
+
+def _queue() -> int:
+    """the current stream of the current device, as _stream, without making a stream object"""
+    return _raw_stream(_device_index())
 
 
 def _dtype(t: torch.dtype) -> int:
@@ -423,23 +431,32 @@ def _dtype(t: torch.dtype) -> int:
     return d
 
 
-def _rows(t: torch.Tensor, what: str) -> torch.Tensor:
-    """a CUDA tensor of rows: unit stride along the last dimension"""
+def _rows(t: torch.Tensor, what: str) -> tuple[int, int, int]:
+    """(rows, columns, row stride) of a 2-D CUDA tensor with unit stride along its rows"""
     if not t.is_cuda:
         raise ValueError("fufft_b200 operates on CUDA tensors")
-    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1) or (t.stride(0) < t.shape[1] and t.shape[0] > 1):
-        raise ValueError(f"{what} must be a 2-D tensor with unit stride along its rows")
-    return t
-
-
-def _row_stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    if t.dim() == 2:
+        (rows, cols), (pitch, unit) = t.shape, t.stride()
+        if rows <= 1:
+            pitch = cols
+        if (unit == 1 or cols <= 1) and pitch >= cols:
+            return rows, cols, pitch
+    raise ValueError(f"{what} must be a 2-D tensor with unit stride along its rows")
 
 
 def _i32(t: torch.Tensor, n: int, what: str):
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n:
+    if t.dtype != torch.int32 or t.shape != (n,):
         raise ValueError(f"{what} must be int32 with {n} entries")
     return _ptr(t)
+
+
+def _result(out: torch.Tensor | None, like: torch.Tensor, rows: int, cols: int, dtype: torch.dtype) -> tuple[torch.Tensor, int]:
+    """a [rows, cols] result and its row stride: the caller's `out`, or a new one on like's device"""
+    if out is None:
+        return like.new_empty((rows, cols), dtype=dtype), cols
+    if out.dtype != dtype or out.shape != (rows, cols):
+        raise ValueError(f"out must be {dtype} {(rows, cols)}")
+    return out, _rows(out, "out")[2]
 
 
 class Mx4:
@@ -447,38 +464,58 @@ class Mx4:
     codes uint8 [rows, ceil(cols / 256) * 128] and the tiled E8M0 scales uint8
     [ceil(rows / 128), ceil(cols / 256) * 2, 32, 4, 4] (layout in
     include/fufft_b200.h, fufft_mx4_*)"""
-    __slots__ = ("codes", "scales", "rows", "cols")
+    __slots__ = ("_codes", "_scales", "_buffer", "rows", "cols", "at")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, cols: int):
-        tiles = -(-cols // 256) * 2
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
             raise TypeError("codes and scales must be uint8")
+        tiles = -(-cols // 256) * 2
         if codes.numel() != rows * tiles * 64 or scales.numel() != -(-rows // 128) * tiles * 512:
             raise ValueError(f"codes or scales do not fit a {rows} x {cols} matrix")
-        self.codes, self.scales, self.rows, self.cols = codes, scales, rows, cols
+        self._codes, self._scales, self._buffer, self.rows, self.cols = codes, scales, codes, rows, cols
+        self.at = _ptr(codes), _ptr(scales)
+
+    @property
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            pitch = -(-self.cols // 256) * 128
+            self._codes = self._buffer[: self.rows * pitch].view(self.rows, pitch)
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            row_tiles, tiles = -(-self.rows // 128), -(-self.cols // 256) * 2
+            at = self._buffer.numel() - row_tiles * tiles * 512
+            self._scales = self._buffer[at:].view(row_tiles, tiles, 32, 4, 4)
+        return self._scales
 
     @property
     def shape(self) -> tuple[int, int]:
         return self.rows, self.cols
 
 
+def _mx4_new(like: torch.Tensor, rows: int, cols: int) -> Mx4:
+    """uninitialised: codes, then scales, in one buffer on like's device"""
+    q = Mx4.__new__(Mx4)
+    tiles = -(-cols // 256) * 2
+    codes = rows * tiles * 64          # a multiple of 128
+    q._buffer = like.new_empty(codes + -(-rows // 128) * tiles * 512, dtype=torch.uint8)
+    q._codes = q._scales = None
+    q.rows, q.cols = rows, cols
+    at = q._buffer.data_ptr()
+    q.at = at, at + codes
+    return q
+
+
 def mx4_empty(rows: int, cols: int, device=None) -> Mx4:
     """uninitialised buffers of a 4-bit matrix"""
-    tiles = -(-cols // 256) * 2
-    return Mx4(torch.empty(rows, tiles * 64, dtype=torch.uint8, device=device or "cuda"),
-               torch.empty(-(-rows // 128), tiles, 32, 4, 4, dtype=torch.uint8, device=device or "cuda"), rows, cols)
-
-
-def _quantize(x: torch.Tensor, q: Mx4 | None, qt: Mx4 | None) -> None:
-    check(lib().fufft_mx4_quantize(x.data_ptr(), _dtype(x.dtype), x.shape[0], x.shape[1], _row_stride(x),
-                                   None if q is None else _ptr(q.codes), None if q is None else _ptr(q.scales),
-                                   None if qt is None else _ptr(qt.codes), None if qt is None else _ptr(qt.scales),
-                                   _stream()), "fufft_mx4_quantize")
+    return _mx4_new(torch.empty(0, device=device or "cuda"), rows, cols)
 
 
 def _turned(x: torch.Tensor) -> bool:
     """a transposed view: quantised along the other axis of what it is a view of"""
-    return x.is_cuda and x.dim() == 2 and x.stride(0) == 1 and x.stride(1) != 1 and x.shape[0] > 1
+    return x.dim() == 2 and x.stride(0) == 1 and x.stride(1) != 1 and x.shape[0] > 1
 
 
 def mx4_quantize(x: torch.Tensor, transpose: bool = False) -> Mx4:
@@ -486,14 +523,17 @@ def mx4_quantize(x: torch.Tensor, transpose: bool = False) -> Mx4:
     `transpose`, x^T quantised along the columns of x"""
     if _turned(x):
         x, transpose = x.t(), not transpose
-    x = _rows(x, "x")
-    rows, cols = x.shape
+    rows, cols, pitch = _rows(x, "x")
+    dtype = _dtype(x.dtype)
     if transpose:
-        q = mx4_empty(cols, rows, x.device)
-        _quantize(x, None, q)
+        q = _mx4_new(x, cols, rows)
+        at = None, None, *q.at
     else:
-        q = mx4_empty(rows, cols, x.device)
-        _quantize(x, q, None)
+        q = _mx4_new(x, rows, cols)
+        at = *q.at, None, None
+    rc = lib().fufft_mx4_quantize(x.data_ptr(), dtype, rows, cols, pitch, *at, _queue())
+    if rc:
+        check(rc, "fufft_mx4_quantize")
     return q
 
 
@@ -501,21 +541,29 @@ def mx4_quantize_both(x: torch.Tensor) -> tuple[Mx4, Mx4]:
     """(mx4_quantize(x), mx4_quantize(x, transpose=True)) from one read of x"""
     if _turned(x):
         return mx4_quantize_both(x.t())[::-1]
-    x = _rows(x, "x")
-    q, qt = mx4_empty(x.shape[0], x.shape[1], x.device), mx4_empty(x.shape[1], x.shape[0], x.device)
-    _quantize(x, q, qt)
+    rows, cols, pitch = _rows(x, "x")
+    dtype = _dtype(x.dtype)
+    q, qt = _mx4_new(x, rows, cols), _mx4_new(x, cols, rows)
+    rc = lib().fufft_mx4_quantize(x.data_ptr(), dtype, rows, cols, pitch, *q.at, *qt.at, _queue())
+    if rc:
+        check(rc, "fufft_mx4_quantize")
     return q, qt
 
 
 def mx4_dequantize(q: Mx4, dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None) -> torch.Tensor:
     """the values that q stands for"""
-    if out is None:
-        out = torch.empty(q.rows, q.cols, dtype=dtype, device=q.codes.device)
-    elif out.dtype != dtype or out.shape != q.shape:
-        raise ValueError(f"out must be {dtype} {q.shape}")
-    check(lib().fufft_mx4_dequantize(_ptr(q.codes), _ptr(q.scales), q.rows, q.cols, _rows(out, "out").data_ptr(),
-                                     _dtype(dtype), _row_stride(out), _stream()), "fufft_mx4_dequantize")
+    code = _dtype(dtype)
+    out, pitch = _result(out, q._buffer, q.rows, q.cols, dtype)
+    rc = lib().fufft_mx4_dequantize(*q.at, q.rows, q.cols, out.data_ptr(), code, pitch, _queue())
+    if rc:
+        check(rc, "fufft_mx4_dequantize")
     return out
+
+
+def _bias(bias: torch.Tensor | None, n: int):
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,)):
+        raise ValueError(f"bias must be float32 with {n} entries")
+    return _ptr(bias)
 
 
 def mx4_matmul(a: Mx4, b: Mx4, dtype: torch.dtype = torch.bfloat16, bias: torch.Tensor | None = None,
@@ -524,23 +572,33 @@ def mx4_matmul(a: Mx4, b: Mx4, dtype: torch.dtype = torch.bfloat16, bias: torch.
     blocked along the summed axis, bias is float32 [b.rows]"""
     if a.cols != b.cols:
         raise ValueError(f"the summed axes differ: {a.shape} and {b.shape}")
-    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (b.rows,)):
-        raise ValueError(f"bias must be float32 with {b.rows} entries")
-    if out is None:
-        out = torch.empty(a.rows, b.rows, dtype=dtype, device=a.codes.device)
-    elif out.dtype != dtype or out.shape != (a.rows, b.rows):
-        raise ValueError(f"out must be {dtype} {(a.rows, b.rows)}")
-    check(lib().fufft_mx4_matmul(_ptr(a.codes), _ptr(a.scales), _ptr(b.codes), _ptr(b.scales), _ptr(bias),
-                                 _rows(out, "out").data_ptr(), _dtype(dtype), a.rows, b.rows, a.cols,
-                                 _row_stride(out), _stream()), "fufft_mx4_matmul")
+    code = _dtype(dtype)
+    out, pitch = _result(out, a._buffer, a.rows, b.rows, dtype)
+    rc = lib().fufft_mx4_matmul(*a.at, *b.at, _bias(bias, b.rows), out.data_ptr(), code, a.rows, b.rows, a.cols, pitch,
+                                _queue())
+    if rc:
+        check(rc, "fufft_mx4_matmul")
     return out
 
 
 def mx4_linear(x: torch.Tensor, w: Mx4, bias: torch.Tensor | None = None,
                dtype: torch.dtype | None = None) -> torch.Tensor:
     """x [..., k] quantised along k, times w [n, k]: [..., n] in x's dtype unless another is given"""
-    y = mx4_matmul(mx4_quantize(x.reshape(-1, x.shape[-1])), w, dtype or x.dtype, bias)
-    return y.view(*x.shape[:-1], w.rows)
+    flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    if flat.shape[1] != w.cols:
+        raise ValueError(f"the summed axes differ: {tuple(x.shape)} and {w.shape}")
+    if _turned(flat):
+        flat = flat.contiguous()
+    m, k, pitch = _rows(flat, "x")
+    dtype = dtype or x.dtype
+    codes, out_code = _dtype(x.dtype), _dtype(dtype)
+    out = flat.new_empty((m, w.rows), dtype=dtype)
+    q = _mx4_new(flat, m, k)
+    rc = lib().fufft_mx4_linear(flat.data_ptr(), codes, m, k, pitch, *q.at, *w.at, w.rows, _bias(bias, w.rows),
+                                out.data_ptr(), out_code, w.rows, _queue())
+    if rc:
+        check(rc, "fufft_mx4_linear")
+    return out if x.dim() == 2 else out.view(*x.shape[:-1], w.rows)
 
 
 def mx4_linear_grad(gy: torch.Tensor, xt: Mx4, wt: Mx4,
@@ -565,29 +623,25 @@ class SeqCache:
       codes       uint8 [pages, page_size, channels / 2 (mx4) or channels (mx8)]
       scales      uint8 [pages, page_size, channels / 32]
       page_table  int32 [batch, max_pages], -1 where there is no page"""
-    __slots__ = ("codes", "scales", "page_table", "kind", "channels", "desc", "_at")
+    __slots__ = ("codes", "scales", "page_table", "kind", "channels", "batch", "desc", "at")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, page_table: torch.Tensor, kind: str):
-        if kind not in _KINDS:
+        code = _KINDS.get(kind)
+        if code is None:
             raise ValueError(f"kind must be one of {sorted(_KINDS)}")
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or page_table.dtype != torch.int32:
             raise TypeError("codes and scales must be uint8, page_table int32")
-        if codes.dim() != 3 or scales.dim() != 3 or page_table.dim() != 2 or codes.shape[:2] != scales.shape[:2]:
+        if codes.dim() != 3 or scales.dim() != 3 or page_table.dim() != 2:
             raise ValueError("codes and scales must be [pages, page_size, ...], page_table [batch, max_pages]")
+        pages, page_size, width = codes.shape
         channels = scales.shape[2] * 32
-        if codes.shape[2] != (channels // 2 if kind == "mx4" else channels):
-            raise ValueError("codes and scales differ in their channels")
-        if not page_table.is_cuda or (page_table.stride(1) != 1 and page_table.shape[1] > 1):
-            raise ValueError("page_table must be a CUDA tensor with unit stride along its rows")
+        if scales.shape[:2] != (pages, page_size) or width * (2 if code == CACHE_MX4 else 1) != channels:
+            raise ValueError("codes and scales differ in their pages or channels")
+        self.batch, max_pages, stride = _rows(page_table, "page_table")
         self.codes, self.scales, self.page_table, self.kind, self.channels = codes, scales, page_table, kind, channels
-        stride = page_table.stride(0) if page_table.shape[0] > 1 else page_table.shape[1]
-        self.desc = CacheDesc(_ptr(codes), _ptr(scales), page_table.data_ptr(), stride, _KINDS[kind], channels,
-                              codes.shape[1], codes.shape[0], page_table.shape[1], page_table.shape[0])
-        self._at = ct.addressof(self.desc)
-
-    @property
-    def batch(self) -> int:
-        return self.page_table.shape[0]
+        self.desc = CacheDesc(_ptr(codes), _ptr(scales), page_table.data_ptr(), stride, code, channels, page_size, pages,
+                              max_pages, self.batch)
+        self.at = ct.addressof(self.desc)
 
 
 def seq_cache(pages: int, page_size: int, channels: int, page_table: torch.Tensor, kind: str = "mx8") -> SeqCache:
@@ -602,26 +656,26 @@ def seq_cache(pages: int, page_size: int, channels: int, page_table: torch.Tenso
 def cache_append(cache: SeqCache, x: torch.Tensor, cu: torch.Tensor, starts: torch.Tensor) -> None:
     """quantise the tokens x [tokens, channels] into the cache: tokens
     cu[b] .. cu[b + 1] - 1 go to sequence b from position starts[b] on"""
-    x = _rows(x, "x")
-    if x.shape[1] != cache.channels:
+    tokens, channels, pitch = _rows(x, "x")
+    if channels != cache.channels:
         raise ValueError(f"x must have {cache.channels} channels")
-    check(lib().fufft_cache_append(cache._at, x.data_ptr(), _dtype(x.dtype), _row_stride(x),
-                                   _i32(cu, cache.batch + 1, "cu"), _i32(starts, cache.batch, "starts"), x.shape[0],
-                                   _stream()), "fufft_cache_append")
+    rc = lib().fufft_cache_append(cache.at, x.data_ptr(), _dtype(x.dtype), pitch, _i32(cu, cache.batch + 1, "cu"),
+                                  _i32(starts, cache.batch, "starts"), tokens, _queue())
+    if rc:
+        check(rc, "fufft_cache_append")
 
 
 def cache_read(cache: SeqCache, cu: torch.Tensor, starts: torch.Tensor, tokens: int,
                dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None) -> torch.Tensor:
     """stored values [tokens, channels] of the ragged run (cu, starts), as in cache_append"""
-    if out is None:
-        out = torch.empty(tokens, cache.channels, dtype=dtype, device=cache.codes.device)
-    elif out.dtype != dtype or out.shape != (tokens, cache.channels):
-        raise ValueError(f"out must be {dtype} {(tokens, cache.channels)}")
+    code = _dtype(dtype)
+    out, pitch = _result(out, cache.codes, tokens, cache.channels, dtype)
     if cache.batch == 0:
         out.zero_()
-    check(lib().fufft_cache_read(cache._at, _rows(out, "out").data_ptr(), _dtype(dtype), _row_stride(out),
-                                 _i32(cu, cache.batch + 1, "cu"), _i32(starts, cache.batch, "starts"), tokens,
-                                 _stream()), "fufft_cache_read")
+    rc = lib().fufft_cache_read(cache.at, out.data_ptr(), code, pitch, _i32(cu, cache.batch + 1, "cu"),
+                                _i32(starts, cache.batch, "starts"), tokens, _queue())
+    if rc:
+        check(rc, "fufft_cache_read")
     return out
 
 
@@ -630,10 +684,12 @@ def cache_read_channels(cache: SeqCache, starts: torch.Tensor, counts: torch.Ten
     """[batch, channels, n]: positions starts[b] .. starts[b] + counts[b] - 1 of
     every sequence, channel by channel, zeros from counts[b] on -- two of
     these rows are what conv_r2 takes"""
-    out = torch.empty(cache.batch, cache.channels, n, dtype=dtype, device=cache.codes.device)
-    check(lib().fufft_cache_read_channels(cache._at, out.data_ptr(), _dtype(dtype), n,
-                                          _i32(starts, cache.batch, "starts"), _i32(counts, cache.batch, "counts"),
-                                          _stream()), "fufft_cache_read_channels")
+    code = _dtype(dtype)
+    out = cache.codes.new_empty((cache.batch, cache.channels, n), dtype=dtype)
+    rc = lib().fufft_cache_read_channels(cache.at, out.data_ptr(), code, n, _i32(starts, cache.batch, "starts"),
+                                         _i32(counts, cache.batch, "counts"), _queue())
+    if rc:
+        check(rc, "fufft_cache_read_channels")
     return out
 
 
@@ -644,23 +700,23 @@ def cache_conv(cache: SeqCache, lengths: torch.Tensor, taps: torch.Tensor, gate:
     gate[b, c] * sum_j taps[j, c // (channels // heads)] * x[b, lengths[b] - 1 - j, c]
     over j < min(lengths[b], len(taps)); taps [n_taps, heads] float32 or
     bfloat16, gate [batch, channels] of `dtype` or None"""
-    taps = _rows(taps, "taps")
+    n, heads, taps_pitch = _rows(taps, "taps")
     if taps.dtype not in (torch.float32, torch.bfloat16):
         raise TypeError("taps must be float32 or bfloat16")
-    if out is None:
-        out = torch.empty(cache.batch, cache.channels, dtype=dtype, device=cache.codes.device)
-    elif out.dtype != dtype or out.shape != (cache.batch, cache.channels):
-        raise ValueError(f"out must be {dtype} {(cache.batch, cache.channels)}")
-    if gate is not None and (gate.dtype != dtype or gate.shape != out.shape):
-        raise ValueError(f"gate must be {dtype} {tuple(out.shape)}")
+    code = _dtype(dtype)
+    out, pitch = _result(out, cache.codes, cache.batch, cache.channels, dtype)
+    gate_at, gate_pitch = None, 0
+    if gate is not None:
+        if gate.dtype != dtype or gate.shape != out.shape:
+            raise ValueError(f"gate must be {dtype} {tuple(out.shape)}")
+        gate_at, gate_pitch = gate.data_ptr(), _rows(gate, "gate")[2]
     if workspace is None:
-        need = lib().fufft_cache_conv_workspace(cache._at, taps.shape[0])
+        need = lib().fufft_cache_conv_workspace(cache.at, n)
         if need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=out.device)
-    check(lib().fufft_cache_conv(cache._at, _i32(lengths, cache.batch, "lengths"), taps.data_ptr(), _dtype(taps.dtype),
-                                 taps.shape[0], taps.shape[1], _row_stride(taps),
-                                 None if gate is None else _rows(gate, "gate").data_ptr(),
-                                 0 if gate is None else _row_stride(gate), _rows(out, "out").data_ptr(), _dtype(dtype),
-                                 _row_stride(out), _ptr(workspace), 0 if workspace is None else workspace.numel(),
-                                 _stream()), "fufft_cache_conv")
+            workspace = out.new_empty(need, dtype=torch.uint8)
+    rc = lib().fufft_cache_conv(cache.at, _i32(lengths, cache.batch, "lengths"), taps.data_ptr(), _DTYPES[taps.dtype], n,
+                                heads, taps_pitch, gate_at, gate_pitch, out.data_ptr(), code, pitch, _ptr(workspace),
+                                0 if workspace is None else workspace.numel(), _queue())
+    if rc:
+        check(rc, "fufft_cache_conv")
     return out

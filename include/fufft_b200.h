@@ -429,6 +429,13 @@ fufft_status fufft_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, i
 fufft_status fufft_mx4_matmul(const uint8_t* a_codes, const uint8_t* a_scales, const uint8_t* b_codes,
                               const uint8_t* b_scales, const float* bias, void* out, fufft_dtype dtype, int64_t m,
                               int64_t n, int64_t k, int64_t out_stride, fufft_stream_t stream);
+/* linear: the two in one call, out = Q(x) w^T + bias with x [m][k] as for
+ * quantize and w [n][k]; x_codes / x_scales (buffers of an m x k matrix) are
+ * left with Q(x). */
+fufft_status fufft_mx4_linear(const void* x, fufft_dtype x_dtype, int64_t m, int64_t k, int64_t x_stride,
+                              uint8_t* x_codes, uint8_t* x_scales, const uint8_t* w_codes, const uint8_t* w_scales,
+                              int64_t n, const float* bias, void* out, fufft_dtype dtype, int64_t out_stride,
+                              fufft_stream_t stream);
 
 /* ---- quantised sequence cache (no reference counterpart) -----------------
  * The past inputs of `batch` sequences in pages of page_size tokens, each
