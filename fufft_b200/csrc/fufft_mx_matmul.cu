@@ -34,6 +34,7 @@ struct MatmulArgs {
 // summed axis and join their sums through distributed shared memory, in rank
 // order.  Bound by reading b's codes and scales once.
 // ---------------------------------------------------------------------------
+constexpr int MAX_SPLIT = 8;         // CTAs of a portable cluster
 template<int BN> struct Split {
    static constexpr int SF_Q = (BN + 127) / 128;                     // scale tiles of the columns
    static constexpr int P_BYTES = 128 * 128, Q_BYTES = BN * 128, SF_BYTES = 1024;
@@ -42,7 +43,7 @@ template<int BN> struct Split {
    static constexpr int SF_COLS = 8 + 8 * SF_Q;                      // tensor-memory columns of a stage's scales
    static constexpr int NEED = BN + STAGES * SF_COLS;
    static constexpr int TMEM = NEED <= 128 ? 128 : NEED <= 256 ? 256 : 512;
-   static constexpr int PITCH = 129;                                 // of a partial column, in floats
+   static constexpr int PITCH = 132;                                 // of a partial column, in floats
    static constexpr int JOIN = BN * PITCH * 4;
    static constexpr int BODY = STAGES * STAGE > JOIN ? STAGES * STAGE : JOIN;
    static constexpr int SMEM = BODY + 1024 + 128;
@@ -61,7 +62,7 @@ __global__ void __launch_bounds__(128) matmul_split_kernel(const __grid_constant
    uint64_t* done = empty + C::STAGES;
    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(done + 1);
 
-   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+   const int warp = tc::uniform_warp(), lane = threadIdx.x & 31;
    const int rank = g.split > 1 ? (int)tc::cluster_rank() : 0;
    const long long tile = blockIdx.x / g.split;
    const int p0 = (int)(tile % g.tiles_p) * 128;
@@ -85,58 +86,87 @@ __global__ void __launch_bounds__(128) matmul_split_kernel(const __grid_constant
    tc::fence_before_sync();
    __syncthreads();
    tc::fence_after_sync();
-   const uint32_t tmem = *tmem_at;
+   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_at, 0);
 
-   if(threadIdx.x == 0) {
+   if(warp == 0) {
       // copies: both operands' 256 columns and their scales, one stage each
       const long long q_tile_last = ceil_div(g.q_rows, TILE_ROWS) - 1;
-      int issued = 0;
+      const uint8_t* p_scale = g.p_scale + ((long long)(p0 / TILE_ROWS) * g.chunks + k0) * C::SF_BYTES;
+      const uint8_t* q_scale = g.q_scale + (q0 / TILE_ROWS * g.chunks + k0) * C::SF_BYTES;
+      auto load_p = [&](int i, int s) {
+         mbar_expect_tx(full + s, C::STAGE);
+         tma_load_2d(body + s * C::STAGE, &tp, (k0 + i) * 128, p0, full + s);
+         bulk_g2s(body + s * C::STAGE + C::P_BYTES + C::Q_BYTES, p_scale + (long long)i * C::SF_BYTES, C::SF_BYTES, full + s);
+      };
+      auto load_q = [&](int i, int s) {
+         uint8_t* at = body + s * C::STAGE + C::P_BYTES;
+         tma_load_2d(at, &tq, (k0 + i) * 128, (int)q0, full + s);
+#pragma unroll
+         for(int h = 0; h < C::SF_Q; ++h)
+            bulk_g2s(at + C::Q_BYTES + (1 + h) * C::SF_BYTES,
+                     q_scale + (min((long long)h, q_tile_last - q0 / TILE_ROWS) * g.chunks + i) * C::SF_BYTES, C::SF_BYTES, full + s);
+      };
+      // b's first stages are under way before a's quantisation, the kernel before, has ended
+      const int ahead = min(n, C::STAGES);
+      if(tc::elect())
+         for(int i = 0; i < ahead; ++i) load_p(i, i);
+      tc::wait_for_previous();
+      if(tc::elect())
+         for(int i = 0; i < ahead; ++i) load_q(i, i);
+      __syncwarp();
+      int issued = ahead, s = 0;
+      uint32_t phase = 0;
       bool ok = true;
-      for(int i = 0; i < n && ok; ++i) {
-         const int s = i % C::STAGES;
-         if(!mbar_wait(empty + s, (i / C::STAGES & 1) ^ 1, g.status)) {
+      for(int i = ahead; i < n; ++i) {
+         if(!mbar_wait(empty + s, phase, g.status)) {
             ok = false;
             break;
          }
-         uint8_t* at = body + s * C::STAGE;
-         mbar_expect_tx(full + s, C::STAGE);
-         tma_load_2d(at, &tp, (k0 + i) * 128, p0, full + s);
-         tma_load_2d(at + C::P_BYTES, &tq, (k0 + i) * 128, (int)q0, full + s);
-         at += C::P_BYTES + C::Q_BYTES;
-         bulk_g2s(at, g.p_scale + ((long long)(p0 / TILE_ROWS) * g.chunks + k0 + i) * C::SF_BYTES, C::SF_BYTES, full + s);
-         for(int h = 0; h < C::SF_Q; ++h) {
-            const long long row_tile = min(q0 / TILE_ROWS + h, q_tile_last);
-            bulk_g2s(at + (1 + h) * C::SF_BYTES, g.q_scale + (row_tile * g.chunks + k0 + i) * C::SF_BYTES, C::SF_BYTES, full + s);
+         if(tc::elect()) {
+            load_p(i, s);
+            load_q(i, s);
          }
+         __syncwarp();
          issued = i + 1;
+         if(++s == C::STAGES) {
+            s = 0;
+            phase ^= 1;
+         }
       }
       // after a wait that gave up: no copy may still be landing when the CTA ends
       if(!ok)
          for(int i = max(0, issued - C::STAGES); i < issued; ++i) mbar_wait(full + i % C::STAGES, i / C::STAGES & 1, g.status);
-   } else if(threadIdx.x == 32 && n > 0) {
-      const uint32_t sf_at = tmem + BN;
+   } else if(warp == 1 && n > 0) {
       const uint32_t q_col = (uint32_t)(q0 % TILE_ROWS / 32);       // this tile's first scale column of its row tile
+      const uint64_t rows0 = tc::rows_desc(smem_u32(body)), scales0 = tc::scales_desc(smem_u32(body) + C::P_BYTES + C::Q_BYTES);
+      int s = 0;
+      uint32_t phase = 0;
       for(int i = 0; i < n; ++i) {
-         const int s = i % C::STAGES;
-         if(!mbar_wait(full + s, i / C::STAGES & 1, g.status)) break;
+         if(!mbar_wait(full + s, phase, g.status)) break;
          tc::fence_after_sync();
-         const uint32_t at = smem_u32(body + s * C::STAGE), sf = at + C::P_BYTES + C::Q_BYTES;
-         const uint32_t col = sf_at + s * C::SF_COLS;
+         const uint64_t rows = rows0 + (uint32_t)(s * (C::STAGE >> 4)), sf = scales0 + (uint32_t)(s * (C::STAGE >> 4));
+         const uint32_t col = tmem + BN + s * C::SF_COLS;
+         if(tc::elect()) {
 #pragma unroll
-         for(int t = 0; t < 2; ++t) {
-            tc::copy_scales(col + t * 4, tc::scales_desc(sf + t * TILE_BYTES));
+            for(int t = 0; t < 2; ++t) {
+               tc::copy_scales(col + t * 4, sf + t * (TILE_BYTES >> 4));
 #pragma unroll
-            for(int h = 0; h < C::SF_Q; ++h)
-               tc::copy_scales(col + 8 + (t * C::SF_Q + h) * 4, tc::scales_desc(sf + (1 + h) * C::SF_BYTES + t * TILE_BYTES));
+               for(int h = 0; h < C::SF_Q; ++h)
+                  tc::copy_scales(col + 8 + (t * C::SF_Q + h) * 4, sf + (((1 + h) * C::SF_BYTES + t * TILE_BYTES) >> 4));
+            }
+#pragma unroll
+            for(int k = 0; k < 4; ++k)
+               tc::mma_mxf4(tmem, rows + k * 2, rows + ((C::P_BYTES + k * 32) >> 4), tc::mxf4_idesc(128, BN, (k & 1) * 2),
+                            col + (k >> 1) * 4, col + 8 + (k >> 1) * C::SF_Q * 4 + q_col, i > 0 || k > 0);
+            tc::commit(empty + s);
          }
-#pragma unroll
-         for(int k = 0; k < 4; ++k)
-            tc::mma_mxf4(tmem, tc::rows_desc(at + k * 32), tc::rows_desc(at + C::P_BYTES + k * 32),
-                         tc::mxf4_idesc(128, BN, (k & 1) * 2), col + (k >> 1) * 4, col + 8 + (k >> 1) * C::SF_Q * 4 + q_col,
-                         i > 0 || k > 0);
-         tc::commit(empty + s);
+         __syncwarp();
+         if(++s == C::STAGES) {
+            s = 0;
+            phase ^= 1;
+         }
       }
-      tc::commit(done);
+      if(tc::elect()) tc::commit(done);
    }
    __syncwarp();
    bool ok = n == 0 || mbar_wait(done, 0, g.status);
@@ -169,15 +199,27 @@ __global__ void __launch_bounds__(128) matmul_split_kernel(const __grid_constant
          for(int j = 0; j < 16; ++j) part[(j0 + j) * C::PITCH + line] = n && ok ? v[j] : 0.0f;
       }
       tc::cluster_sync();
+      // a warp takes a column, a lane four rows of b: the ranks' sums are loaded side by side, added in order
       const int rows = (int)min((long long)BN, g.q_rows - q0);
-      const long long row = p0 + threadIdx.x;
-      if(row < g.p_rows) {
-         const float bias = g.bias ? g.bias[row] : 0.0f;
-         for(int j = rank; j < rows; j += g.split) {
-            float sum = 0.0f;
-            for(int r = 0; r < g.split; ++r) sum += tc::load_peer(tc::peer_smem(part + j * C::PITCH + threadIdx.x, r));
-            out[(q0 + j) * g.out_stride + row] = from_f<T>(sum + bias);
-         }
+      const long long row = p0 + lane * 4;
+      for(int j = rank * 4 + warp; j < rows; j += g.split * 4) {
+         float4 v[MAX_SPLIT];
+#pragma unroll
+         for(int r = 0; r < MAX_SPLIT; ++r)
+            if(r < g.split) v[r] = tc::load_peer4(tc::peer_smem(part + j * C::PITCH + lane * 4, r));
+         float4 sum = v[0];
+#pragma unroll
+         for(int r = 1; r < MAX_SPLIT; ++r)
+            if(r < g.split) {
+               sum.x += v[r].x;
+               sum.y += v[r].y;
+               sum.z += v[r].z;
+               sum.w += v[r].w;
+            }
+         const float y[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+         for(int x = 0; x < 4; ++x)
+            if(row + x < g.p_rows) out[(q0 + j) * g.out_stride + row + x] = from_f<T>(y[x] + (g.bias ? g.bias[row + x] : 0.0f));
       }
       tc::cluster_sync();   // nobody leaves while its sums are being read
    }
@@ -186,8 +228,231 @@ __global__ void __launch_bounds__(128) matmul_split_kernel(const __grid_constant
    if(warp == 2) tc::tmem_free<C::TMEM>(tmem);
 }
 
-// 128-byte rows of 4-bit codes, `rows` of them `pitch` bytes apart
-fufft_status codes_tmap(CUtensorMap* tm, const uint8_t* codes, long long rows, long long pitch, int box_rows)
+// ---------------------------------------------------------------------------
+// Many outputs: pairs of CTAs, 256 rows of one operand by BN of the other a
+// tile, each CTA holding half of both; a pair walks over tiles.  One warp
+// copies, one issues, eight bring the finished sums out.  The 256 rows
+// (tensor-memory lanes) are a's, and a lane stores whole sectors of its row
+// of the result, where those rows start on 32 bytes; else they are b's
+// (SWAP), and the lanes of a warp store side by side, aligned or not.
+// ---------------------------------------------------------------------------
+template<int BN_, int ACC_> struct Pair {
+   static constexpr int BN = BN_, ACC = ACC_;                        // columns of a tile; accumulators
+   static constexpr int STAGES = 5;
+   static constexpr int A_BYTES = 128 * 128, B_BYTES = BN / 2 * 128, SF_BYTES = 1024;
+   static constexpr int STAGE = A_BYTES + B_BYTES + 3 * SF_BYTES;    // scales: 128 rows of a, 256 rows of b
+   static constexpr int SF_COLS = 24;
+   static constexpr int SF_AT = ACC * BN;
+   static constexpr int TMEM = 512;
+   static constexpr int SMEM = STAGES * STAGE + 1024 + 256;
+   static constexpr int THREADS = 320, EPILOGUE = 8;
+   static constexpr int COLS = BN / 2;                               // a warp of the epilogue holds 32 x COLS
+   static constexpr int GROUP = 8;                                   // row tiles that are walked together
+   static_assert(STAGE % 1024 == 0 && SF_AT + STAGES * SF_COLS <= TMEM && BN % 32 == 0 && BN <= 256, "tile");
+};
+
+struct PairArgs {
+   const float* bias;
+   void* out;
+   unsigned int* status;
+   long long m, n, out_stride;
+   int chunks, tiles_m, tiles_n;
+};
+
+// N consecutive results of one row, `left` of which exist, in whole 32-byte sectors
+template<class T, int N>
+__device__ __forceinline__ void store_row(T* at, const float* v, const float* bias, long long left)
+{
+   constexpr int W = 32 / (int)sizeof(T);
+#pragma unroll
+   for(int j = 0; j < N; j += W) {
+      float x[W];
+#pragma unroll
+      for(int i = 0; i < W; ++i) x[i] = v[j + i] + (bias && j + i < left ? __ldg(bias + j + i) : 0.0f);
+      if(j + W <= left) {
+         uint32_t w[8];
+#pragma unroll
+         for(int i = 0; i < 8; ++i) {
+            if constexpr(sizeof(T) == 4) w[i] = __float_as_uint(x[i]);
+            else w[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
+         }
+         asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                      :: "l"(at + j), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                      : "memory");
+      } else {
+#pragma unroll
+         for(int i = 0; i < W; ++i)
+            if(j + i < left) at[j + i] = from_f<T>(x[i]);
+      }
+   }
+}
+
+template<class P> __device__ __forceinline__ void pair_tile(const PairArgs& g, long long t, int* m0, int* n0)
+{
+   const long long per = (long long)P::GROUP * g.tiles_n;
+   const int first = (int)(t / per) * P::GROUP, rows = min(P::GROUP, g.tiles_m - first);
+   const int in = (int)(t % per);
+   *m0 = (first + in % rows) * 256;
+   *n0 = in / rows * P::BN;
+}
+
+template<class T, class P, bool SWAP>
+__global__ void __launch_bounds__(P::THREADS, 1) matmul_pair_kernel(const __grid_constant__ CUtensorMap ta,
+                                                                    const __grid_constant__ CUtensorMap tb,
+                                                                    const __grid_constant__ CUtensorMap tsa,
+                                                                    const __grid_constant__ CUtensorMap tsb, PairArgs g)
+{
+   extern __shared__ uint8_t raw[];
+   uint8_t* body = reinterpret_cast<uint8_t*>(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+   uint64_t* full = reinterpret_cast<uint64_t*>(body + P::STAGES * P::STAGE);   // in the even CTA: both halves have landed
+   uint64_t* empty = full + P::STAGES;                                         // in each: the products have read the stage
+   uint64_t* ready = empty + P::STAGES;                                        // in each: an accumulator is summed
+   uint64_t* taken = ready + P::ACC;                                           // in the even CTA: both have read it
+   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(taken + P::ACC);
+
+   const int warp = tc::uniform_warp(), lane = threadIdx.x & 31;
+   const uint32_t rank = tc::cluster_rank();
+   const long long tiles = (long long)g.tiles_m * g.tiles_n, first = blockIdx.x >> 1, step = gridDim.x >> 1;
+
+   if(threadIdx.x == 0) {
+      for(int s = 0; s < P::STAGES; ++s) {
+         mbar_init(full + s, 1);
+         mbar_init(empty + s, 1);
+      }
+      for(int s = 0; s < P::ACC; ++s) {
+         mbar_init(ready + s, 1);
+         mbar_init(taken + s, 2 * P::EPILOGUE);
+      }
+      fence_mbar_init();
+      prefetch_tmap(&ta);
+      prefetch_tmap(&tb);
+      prefetch_tmap(&tsa);
+      prefetch_tmap(&tsb);
+   }
+   if(warp == 1) tc::tmem_alloc_pair<P::TMEM>(tmem_at);
+   tc::fence_before_sync();
+   tc::cluster_sync();
+   tc::fence_after_sync();
+   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_at, 0);
+
+   if(warp == 0) {
+      bool ok = true;
+      int s = 0;
+      uint32_t phase = 1;
+      tc::wait_for_previous();
+      for(long long t = first; t < tiles && ok; t += step) {
+         int m0, n0;
+         pair_tile<P>(g, t, &m0, &n0);
+         const int a_row = m0 + (int)rank * 128, b_row = n0 + (int)rank * (P::BN / 2);
+         const int a_tile = m0 / TILE_ROWS + (int)rank, b_tile = n0 / TILE_ROWS;
+         for(int k = 0; k < g.chunks; ++k) {
+            if(!mbar_wait(empty + s, phase, g.status)) {
+               ok = false;
+               break;
+            }
+            if(tc::elect()) {
+               uint8_t* at = body + s * P::STAGE;
+               const uint32_t bar = tc::peer_smem(full + s, 0);
+               if(rank == 0) mbar_expect_tx(full + s, 2 * P::STAGE);
+               tc::tma_load_2d_pair(at, &ta, k * 128, a_row, bar);
+               tc::tma_load_2d_pair(at + P::A_BYTES, &tb, k * 128, b_row, bar);
+               at += P::A_BYTES + P::B_BYTES;
+               tc::tma_load_2d_pair(at, &tsa, k * 256, a_tile, bar);
+               tc::tma_load_2d_pair(at + P::SF_BYTES, &tsb, k * 256, b_tile, bar);
+               tc::tma_load_2d_pair(at + 2 * P::SF_BYTES, &tsb, k * 256, b_tile + 1, bar);
+            }
+            __syncwarp();
+            if(++s == P::STAGES) {
+               s = 0;
+               phase ^= 1;
+            }
+         }
+      }
+      if(!ok) {   // a wait gave up: time for the copies under way, whose barrier may be the other CTA's, to land
+         const uint64_t t0 = globaltimer_ns();
+         while(globaltimer_ns() - t0 < 2000000ull) {}
+      }
+   } else if(warp == 1 && rank == 0) {
+      bool ok = true;
+      int s = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 1;
+      const uint64_t rows0 = tc::rows_desc(smem_u32(body)), scales0 = tc::scales_desc(smem_u32(body) + P::A_BYTES + P::B_BYTES);
+      for(long long t = first; t < tiles && ok; t += step) {
+         int m0, n0;
+         pair_tile<P>(g, t, &m0, &n0);
+         if(!mbar_wait<true>(taken + acc, acc_phase, g.status)) break;
+         tc::fence_after_sync();
+         const uint32_t d = tmem + acc * P::BN, b_col = (uint32_t)(n0 % TILE_ROWS / 32);
+         for(int k = 0; k < g.chunks; ++k) {
+            if(!mbar_wait<true>(full + s, phase, g.status)) {
+               ok = false;
+               break;
+            }
+            tc::fence_after_sync();
+            const uint64_t rows = rows0 + (uint32_t)(s * (P::STAGE >> 4)), sf = scales0 + (uint32_t)(s * (P::STAGE >> 4));
+            const uint32_t col = tmem + P::SF_AT + s * P::SF_COLS;
+            if(tc::elect()) {
+#pragma unroll
+               for(int h = 0; h < 2; ++h) {
+                  tc::copy_scales_pair(col + h * 4, sf + h * (TILE_BYTES >> 4));
+                  tc::copy_scales_pair(col + 8 + h * 8, sf + ((P::SF_BYTES + h * TILE_BYTES) >> 4));
+                  tc::copy_scales_pair(col + 12 + h * 8, sf + ((2 * P::SF_BYTES + h * TILE_BYTES) >> 4));
+               }
+#pragma unroll
+               for(int q = 0; q < 4; ++q)
+                  tc::mma_mxf4_pair(d, rows + q * 2, rows + ((P::A_BYTES + q * 32) >> 4), tc::mxf4_idesc(256, P::BN, (q & 1) * 2),
+                                    col + (q >> 1) * 4, col + 8 + (q >> 1) * 8 + b_col, k > 0 || q > 0);
+               tc::commit_pair(empty + s);
+               if(k + 1 == g.chunks) tc::commit_pair(ready + acc);
+            }
+            __syncwarp();
+            if(++s == P::STAGES) {
+               s = 0;
+               phase ^= 1;
+            }
+         }
+         if(++acc == P::ACC) {
+            acc = 0;
+            acc_phase ^= 1;
+         }
+      }
+   } else if(warp >= 2) {
+      const int quarter = warp & 3, half = (warp - 2) / 4;   // the lanes that this warp may read; its columns
+      long long done = 0;
+      T* out = static_cast<T*>(g.out);
+      for(long long t = first; t < tiles; t += step, ++done) {
+         int m0, n0;
+         pair_tile<P>(g, t, &m0, &n0);
+         const int acc = (int)(done % P::ACC);
+         if(!mbar_wait<true>(ready + acc, (uint32_t)(done / P::ACC & 1), g.status)) break;
+         tc::fence_after_sync();
+         const uint32_t mine = tmem + ((uint32_t)quarter << 21) + acc * P::BN + half * P::COLS;
+         float v[P::COLS];
+         __syncwarp();   // rows beyond the last have skipped their stores
+#pragma unroll
+         for(int j = 0; j < P::COLS; j += 16) tc::tmem_load16(mine + j, v + j);
+         tc::tmem_load_wait();
+         tc::fence_before_sync();
+         __syncwarp();
+         if(lane == 0) tc::arrive_peer(tc::peer_smem(taken + acc, 0));
+         const long long row = m0 + (long long)rank * 128 + quarter * 32 + lane, col = n0 + half * P::COLS;
+         if constexpr(SWAP) {
+            const float bias = g.bias && row < g.m ? g.bias[row] : 0.0f;
+#pragma unroll
+            for(int j = 0; j < P::COLS; ++j)
+               if(row < g.m && col + j < g.n) out[(col + j) * g.out_stride + row] = from_f<T>(v[j] + bias);
+         } else {
+            if(row < g.m && col < g.n) store_row<T, P::COLS>(out + row * g.out_stride + col, v, g.bias ? g.bias + col : nullptr, g.n - col);
+         }
+      }
+   }
+   __syncwarp();
+   tc::fence_before_sync();
+   tc::cluster_sync();       // both have read their sums; nothing is under way in either's memory
+   if(warp == 1) tc::tmem_free_pair<P::TMEM>(tmem);
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 tmap_encoder()
 {
    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
    static std::once_flag once;
@@ -198,6 +463,13 @@ fufft_status codes_tmap(CUtensorMap* tm, const uint8_t* codes, long long rows, l
          q == cudaDriverEntryPointSuccess)
          fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
    });
+   return fn;
+}
+
+// 4-bit codes as tiles of box_rows x 128 bytes, 128-byte swizzle; rows beyond the last read as zeros
+fufft_status codes_tmap(CUtensorMap* tm, const uint8_t* codes, long long rows, long long pitch, int box_rows)
+{
+   const auto fn = tmap_encoder();
    if(!fn) return FUFFT_ERR_UNSUPPORTED;
    cuuint64_t dims[2] = {(cuuint64_t)pitch, (cuuint64_t)rows};
    cuuint64_t strides[1] = {(cuuint64_t)pitch};
@@ -209,11 +481,27 @@ fufft_status codes_tmap(CUtensorMap* tm, const uint8_t* codes, long long rows, l
    return r == CUDA_SUCCESS ? FUFFT_OK : FUFFT_ERR_UNSUPPORTED;
 }
 
+// the scale tiles of 128 rows x 256 columns, 1024 bytes each as 256 words; tiles beyond the last row read as zeros
+fufft_status scales_tmap(CUtensorMap* tm, const uint8_t* scales, long long rows, int chunks)
+{
+   const auto fn = tmap_encoder();
+   if(!fn) return FUFFT_ERR_UNSUPPORTED;
+   cuuint64_t dims[2] = {(cuuint64_t)chunks * 256, (cuuint64_t)ceil_div(rows, TILE_ROWS)};
+   cuuint64_t strides[1] = {(cuuint64_t)chunks * 1024};
+   cuuint32_t box[2] = {256, 1};
+   cuuint32_t estr[2] = {1, 1};
+   const CUresult r = fn(tm, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<uint8_t*>(scales), dims, strides, box, estr,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+   return r == CUDA_SUCCESS ? FUFFT_OK : FUFFT_ERR_UNSUPPORTED;
+}
+
 struct Operands {
    const uint8_t *a, *a_scale, *b, *b_scale;
    const float* bias;
    void* out;
    long long m, n, k, out_stride;
+   bool follows;             // the kernel before on the stream wrote a (and neither b nor anything else that is read)
 };
 
 template<class T, int BN>
@@ -237,12 +525,14 @@ fufft_status launch_split(const Operands& o, int split, const DeviceCtx& ctx, cu
    cfg.blockDim = dim3(128);
    cfg.dynamicSmemBytes = C::SMEM;
    cfg.stream = st;
-   cudaLaunchAttribute at[1];
+   cudaLaunchAttribute at[2];
    at[0].id = cudaLaunchAttributeClusterDimension;
    at[0].val.clusterDim.x = (unsigned)split;
    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+   at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+   at[1].val.programmaticStreamSerializationAllowed = 1;
    cfg.attrs = at;
-   cfg.numAttrs = 1;
+   cfg.numAttrs = o.follows ? 2 : 1;
    if((s = check(cudaLaunchKernelEx(&cfg, kern, tp, tq, g))) != FUFFT_OK) return s;
    count_launch();
    return check(cudaGetLastError());
@@ -252,8 +542,47 @@ fufft_status launch_split(const Operands& o, int split, const DeviceCtx& ctx, cu
 int split_for(long long tiles, int chunks, int sms)
 {
    int split = 1;
-   while(split < 8 && tiles * split * 2 <= 2ll * sms && chunks >= 4 * split) split *= 2;
+   while(split < MAX_SPLIT && tiles * split * 2 <= 2ll * sms && chunks >= 4 * split) split *= 2;
    return split;
+}
+
+template<class T, class P, bool SWAP>
+fufft_status launch_pair(const Operands& o, const DeviceCtx& ctx, cudaStream_t st)
+{
+   const long long pitch = mx4_pitch(o.k);
+   CUtensorMap ta, tb, tsa, tsb;
+   fufft_status s;
+   PairArgs g{o.bias, o.out, ctx.status, o.m, o.n, o.out_stride, (int)(pitch / 128), (int)ceil_div(o.m, 256),
+              (int)ceil_div(o.n, P::BN)};
+   if((s = codes_tmap(&ta, o.a, o.m, pitch, 128)) != FUFFT_OK) return s;
+   if((s = codes_tmap(&tb, o.b, o.n, pitch, P::BN / 2)) != FUFFT_OK) return s;
+   if((s = scales_tmap(&tsa, o.a_scale, o.m, g.chunks)) != FUFFT_OK) return s;
+   if((s = scales_tmap(&tsb, o.b_scale, o.n, g.chunks)) != FUFFT_OK) return s;
+   auto kern = matmul_pair_kernel<T, P, SWAP>;
+   static std::atomic<uint64_t> configured{0};
+   if((s = allow_smem(kern, P::SMEM, configured)) != FUFFT_OK) return s;
+   cudaLaunchConfig_t cfg = {};
+   cfg.gridDim = dim3(2 * (unsigned)std::min<long long>((long long)g.tiles_m * g.tiles_n, sm_count(ctx.device) / 2));
+   cfg.blockDim = dim3(P::THREADS);
+   cfg.dynamicSmemBytes = P::SMEM;
+   cfg.stream = st;
+   cudaLaunchAttribute at[2];
+   at[0].id = cudaLaunchAttributeClusterDimension;
+   at[0].val.clusterDim.x = 2;
+   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+   at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+   at[1].val.programmaticStreamSerializationAllowed = 1;
+   cfg.attrs = at;
+   cfg.numAttrs = o.follows ? 2 : 1;
+   if((s = check(cudaLaunchKernelEx(&cfg, kern, ta, tb, tsa, tsb, g))) != FUFFT_OK) return s;
+   count_launch();
+   return check(cudaGetLastError());
+}
+template<class T, class P> fufft_status launch_pair(const Operands& o, const DeviceCtx& ctx, cudaStream_t st)
+{
+   if(aligned(o.out, 32) && o.out_stride * (long long)sizeof(T) % 32 == 0) return launch_pair<T, P, false>(o, ctx, st);
+   const Operands swapped{o.b, o.b_scale, o.a, o.a_scale, o.bias, o.out, o.n, o.m, o.k, o.out_stride, o.follows};
+   return launch_pair<T, P, true>(swapped, ctx, st);
 }
 
 template<class T> fufft_status matmul(const Operands& o, cudaStream_t st)
@@ -266,7 +595,28 @@ template<class T> fufft_status matmul(const Operands& o, cudaStream_t st)
    if(o.m <= 16) return launch_split<T, 16>(o, split_for(tiles_p, chunks, sms), ctx, st);
    if(o.m <= 32) return launch_split<T, 32>(o, split_for(tiles_p, chunks, sms), ctx, st);
    if(o.m <= 64) return launch_split<T, 64>(o, split_for(tiles_p, chunks, sms), ctx, st);
-   return launch_split<T, 128>(o, split_for(tiles_p * ceil_div(o.m, 128), chunks, sms), ctx, st);
+   // Pairs, unless their tiles leave most of the card idle and a long summed
+   // axis pays for joining its parts (us, split / pair: 512 x 512 x 8192 9.7 /
+   // 13.1, 128 x 1024 x 1024 9.0 / 7.2, 333 x 1537 x 1111 9.4 / 9.1).
+   const long long pairs = sms / 2, narrow = ceil_div(o.m, 256) * ceil_div(o.n, 192), wide = ceil_div(o.m, 256) * ceil_div(o.n, 256);
+   if(narrow * MAX_SPLIT <= pairs && chunks >= 8)
+      return launch_split<T, 128>(o, split_for(tiles_p * ceil_div(o.m, 128), chunks, sms), ctx, st);
+   if(chunks == 0) return launch_split<T, 128>(o, 1, ctx, st);
+   // 256 columns in one accumulator or 192 in two of them, whichever covers the
+   // result in fewer columns' time (us, 256 / 192: 8192^3 189 / 195, 4096^3
+   // 30.9 / 28.5, 512 x 4096 x 4096 11.8 / 10.1)
+   return ceil_div(wide, pairs) * 256 < ceil_div(narrow, pairs) * 192 ? launch_pair<T, Pair<256, 1>>(o, ctx, st)
+                                                                     : launch_pair<T, Pair<192, 2>>(o, ctx, st);
+}
+
+fufft_status matmul(const Operands& o, fufft_dtype dtype, fufft_stream_t stream)
+{
+   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+   switch(dtype) {
+   case FUFFT_F32: return matmul<float>(o, st);
+   case FUFFT_F16: return matmul<__half>(o, st);
+   default: return matmul<__nv_bfloat16>(o, st);
+   }
 }
 
 }  // namespace mx
@@ -298,13 +648,7 @@ fufft_status fufft_mx4_matmul(const uint8_t* a_codes, const uint8_t* a_scales, c
 {
    fufft_status s = check_matmul(a_codes, a_scales, b_codes, b_scales, bias, out, dtype, m, n, k, out_stride);
    if(s != FUFFT_OK || m == 0 || n == 0) return s;
-   const mx::Operands o{a_codes, a_scales, b_codes, b_scales, bias, out, m, n, k, out_stride};
-   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-   switch(dtype) {
-   case FUFFT_F32: return mx::matmul<float>(o, st);
-   case FUFFT_F16: return mx::matmul<__half>(o, st);
-   default: return mx::matmul<__nv_bfloat16>(o, st);
-   }
+   return mx::matmul({a_codes, a_scales, b_codes, b_scales, bias, out, m, n, k, out_stride, false}, dtype, stream);
 }
 
 fufft_status fufft_mx4_linear(const void* x, fufft_dtype x_dtype, int64_t m, int64_t k, int64_t x_stride,
@@ -316,7 +660,7 @@ fufft_status fufft_mx4_linear(const void* x, fufft_dtype x_dtype, int64_t m, int
    fufft_status s = check_matmul(x_codes, x_scales, w_codes, w_scales, bias, out, dtype, m, n, k, out_stride);
    if(s != FUFFT_OK || m == 0 || n == 0) return s;
    if((s = fufft_mx4_quantize(x, x_dtype, m, k, x_stride, x_codes, x_scales, nullptr, nullptr, stream)) != FUFFT_OK) return s;
-   return fufft_mx4_matmul(x_codes, x_scales, w_codes, w_scales, bias, out, dtype, m, n, k, out_stride, stream);
+   return mx::matmul({x_codes, x_scales, w_codes, w_scales, bias, out, m, n, k, out_stride, k > 0}, dtype, stream);
 }
 
 }  // extern "C"

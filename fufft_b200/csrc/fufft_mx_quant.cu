@@ -2,6 +2,7 @@
 // rows, along the columns, or both from one read, and the way back.
 #include "fufft_internal.cuh"
 #include "fufft_mx.cuh"
+#include "fufft_tc.cuh"
 
 using namespace fufft;
 using namespace fufft::host;
@@ -17,6 +18,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict_
                                                             long long row_stride, uint8_t* __restrict__ codes,
                                                             uint8_t* __restrict__ scales, bool vec)
 {
+   tc::let_next_start();
    const int lane = threadIdx.x & 31;
    const long long chunks = mx4_pitch(cols) / (K_PAD / 2);
    const long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);

@@ -76,6 +76,62 @@ __device__ __forceinline__ void commit(uint64_t* bar)
    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(smem_u32(bar)) : "memory");
 }
 
+// ---- the same for a pair of CTAs (cta_group::2): one thread of the even CTA
+// issues for both; A and D rows 0 .. 127 / 128 .. 255 and the halves of B's
+// rows lie in the two CTAs' memories at the same addresses -----------------
+template<int COLS> __device__ __forceinline__ void tmem_alloc_pair(uint32_t* at_smem)
+{
+   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(at_smem)), "n"(COLS) : "memory");
+   asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+}
+template<int COLS> __device__ __forceinline__ void tmem_free_pair(uint32_t at)
+{
+   asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(at), "n"(COLS));
+}
+__device__ __forceinline__ void copy_scales_pair(uint32_t to_tmem, uint64_t desc)
+{
+   asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" :: "r"(to_tmem), "l"(desc) : "memory");
+}
+__device__ __forceinline__ void mma_mxf4_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                              bool add)
+{
+   asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %6, 0;\n\t"
+                "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+                :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"((uint32_t)add) : "memory");
+}
+// completes the barrier at this address in both CTAs
+__device__ __forceinline__ void commit_pair(uint64_t* bar)
+{
+   asm volatile("{\n\t.reg .b16 m;\n\tmov.b16 m, 3;\n\t"
+                "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], m;\n\t}"
+                :: "r"(smem_u32(bar)) : "memory");
+}
+// 2-D tile of this GPU's own memory into this CTA's shared memory, counted on
+// a barrier (cluster address) of either CTA of the pair.  x: a multiple of 16 bytes
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* tm, int x, int y, uint32_t bar)
+{
+   asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                :: "r"(smem_u32(dst)), "l"(tm), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+
+// Tensor instructions take their operands from uniform registers, and the
+// thread that issues them is what a short step waits for: the whole warp runs
+// the issuing loop on values that the compiler sees to be uniform
+// (uniform_warp), and one lane, picked by the hardware, issues.
+__device__ __forceinline__ int uniform_warp() { return __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0); }
+__device__ __forceinline__ bool elect()
+{
+   uint32_t p;
+   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+   return p != 0;
+}
+
+// ---- programmatic dependent launch -----------------------------------------
+// the next kernel of the stream, if it was launched so, may be scheduled from here on
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;"); }
+// everything that the kernel before wrote is there (at once, if this one was launched plainly)
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---- clusters --------------------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_rank()
 {
@@ -95,10 +151,21 @@ __device__ __forceinline__ uint32_t peer_smem(const void* p, uint32_t rank)
    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
    return r;
 }
+__device__ __forceinline__ void arrive_peer(uint32_t bar)
+{
+   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" :: "r"(bar) : "memory");
+}
+// (volatile, but no memory clobber: several may be under way)
 __device__ __forceinline__ float load_peer(uint32_t at)
 {
    float v;
-   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at));
+   return v;
+}
+__device__ __forceinline__ float4 load_peer4(uint32_t at)
+{
+   float4 v;
+   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at));
    return v;
 }
 
