@@ -1,6 +1,8 @@
 // fufft_cache.cu -- the paged sequence cache in microscaled formats: tokens
 // quantised as they are written, read back token by token or channel by
 // channel (zero padded: the rows the FFT convolution takes).
+#include <algorithm>
+
 #include "fufft_cache.cuh"
 
 using namespace fufft;
@@ -22,85 +24,206 @@ __device__ __forceinline__ int find_sequence(const int32_t* cu, int batch, long 
    return lo;
 }
 
-// a thread holds eight channels of a token, four neighbouring threads a block
-template<class T, bool MX8>
-__global__ void __launch_bounds__(256) append_kernel(const T* __restrict__ x, long long row_stride, Pages p,
-                                                     const int32_t* __restrict__ cu, const int32_t* __restrict__ starts,
-                                                     long long tokens, int channels, bool vec)
-{
-   using E = mx::Elem<MX8>;
-   const int per = channels / 8;
-   const long long g = (long long)blockIdx.x * 256 + threadIdx.x;
-   const bool live = g < tokens * per;
-   const long long t = live ? g / per : 0;
-   const int c = live ? (int)(g % per) * 8 : 0;
-   float v[8];
-   mx::load8(x + t * row_stride + c, vec, 8, v);
-   const uint32_t s = mx::block_scale4<E::EMAX>(v);
-   const float inv = mx::scale_inverse(s);
-#pragma unroll
-   for(int i = 0; i < 8; ++i) v[i] = s == 255u ? 0.0f : v[i] * inv;
-   uint32_t w[E::WORDS];
-   E::encode8(v, w);
-   if(!live) return;
-   const int b = find_sequence(cu, p.batch, t);
-   if(b < 0) return;
-   const long long slot = p.slot(b, (long long)starts[b] + (t - cu[b]));
-   if(slot < 0) return;
-   uint32_t* at = reinterpret_cast<uint32_t*>(p.codes + slot * (long long)per * (4 * E::WORDS)) + (c / 8) * E::WORDS;
-   if constexpr(MX8) *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
-   else *at = w[0];
-   if((threadIdx.x & 3) == 0) p.scales[slot * (channels / mx::BLOCK) + c / mx::BLOCK] = (uint8_t)s;
-}
+// A CTA takes `per` tokens: their places are looked up once, by a thread each,
+// then its threads walk over the tokens' halves of blocks (16 channels, two
+// neighbouring lanes a block), a token after the other.  Bound by reading one
+// side and writing the other.
+constexpr int MAX_PER = 64;
+constexpr int THREADS = 256;
 
-template<class T, bool MX8>
-__global__ void __launch_bounds__(256) read_kernel(T* __restrict__ out, long long row_stride, Pages p,
-                                                   const int32_t* __restrict__ cu, const int32_t* __restrict__ starts,
-                                                   long long tokens, int channels, bool vec)
-{
-   using E = mx::Elem<MX8>;
-   const int per = channels / 8;
-   const long long g = (long long)blockIdx.x * 256 + threadIdx.x;
-   if(g >= tokens * per) return;
-   const long long t = g / per;
-   const int c = (int)(g % per) * 8;
-   float v[8] = {};
-   const int b = find_sequence(cu, p.batch, t);
-   const long long slot = b < 0 ? -1 : p.slot(b, (long long)starts[b] + (t - cu[b]));
-   if(slot >= 0) p.load8<MX8>(slot, c, channels, v);
-   mx::store8(out + t * row_stride + c, vec, 8, v);
-}
-
-// a CTA turns 64 positions x 64 channels around in shared memory
-constexpr int RT = 64;
-template<class T, bool MX8>
-__global__ void __launch_bounds__(256) read_channels_kernel(T* __restrict__ out, Pages p,
-                                                            const int32_t* __restrict__ starts,
-                                                            const int32_t* __restrict__ counts, long long n, int channels)
-{
-   __shared__ float tile[RT][RT + 1];
-   const long long tiles_n = (n + RT - 1) / RT, tiles_c = (channels + RT - 1) / RT;
-   const long long id = blockIdx.x;
-   const int b = (int)(id / (tiles_n * tiles_c));
-   const int c0 = (int)(id / tiles_n % tiles_c) * RT;
-   const long long i0 = id % tiles_n * RT;
-   const long long count = counts[b];
-#pragma unroll
-   for(int k = 0; k < RT * RT / 8 / 256; ++k) {
-      const int e = threadIdx.x + 256 * k, r = e / (RT / 8), c = e % (RT / 8) * 8;
-      float v[8] = {};
-      if(i0 + r < count && c0 + c < channels) {
-         const long long slot = p.slot(b, (long long)starts[b] + i0 + r);
-         if(slot >= 0) p.load8<MX8>(slot, c0 + c, channels, v);
+struct Walk {   // over [tokens][units], THREADS at a time, without a division a step
+   unsigned units, dt, du, t, u;
+   __device__ __forceinline__ explicit Walk(unsigned units_)
+      : units(units_), dt(THREADS / units_), du(THREADS % units_), t(threadIdx.x / units_), u(threadIdx.x % units_)
+   {
+   }
+   __device__ __forceinline__ void step()
+   {
+      t += dt;
+      u += du;
+      if(u >= units) {
+         u -= units;
+         ++t;
       }
-#pragma unroll
-      for(int i = 0; i < 8; ++i) tile[r][c + i] = v[i];
+   }
+};
+
+// tokens t0 .. t0 + n - 1: rows of the flattened pages, -1 without one
+__device__ __forceinline__ void look_up(const Pages& p, const int32_t* cu, const int32_t* starts, long long t0, int n,
+                                        int* rows)
+{
+   if(threadIdx.x < n) {
+      const long long t = t0 + threadIdx.x;
+      const int b = find_sequence(cu, p.batch, t);
+      rows[threadIdx.x] = b < 0 ? -1 : (int)p.slot(b, (long long)starts[b] + (t - cu[b]));
    }
    __syncthreads();
-   for(int e = threadIdx.x; e < RT * RT; e += 256) {
-      const int c = e / RT, r = e % RT;
-      if(c0 + c < channels && i0 + r < n) out[((long long)b * channels + c0 + c) * n + i0 + r] = mx::from_f<T>(tile[r][c]);
+}
+
+// four steps' loads, then four steps' stores
+constexpr int U = 4;
+
+template<class T, bool MX8>
+__global__ void __launch_bounds__(THREADS) append_kernel(const T* __restrict__ x, long long row_stride, Pages p,
+                                                         const int32_t* __restrict__ cu, const int32_t* __restrict__ starts,
+                                                         long long tokens, int per, int units, bool on_32)
+{
+   using E = mx::Elem<MX8>;
+   __shared__ int rows[MAX_PER];
+   const long long t0 = (long long)blockIdx.x * per;
+   const int n = (int)min((long long)per, tokens - t0);
+   look_up(p, cu, starts, t0, n, rows);
+   x += t0 * row_stride;
+   Walk w(units);
+   // whole warps go round together: a block's two lanes meet in a shuffle
+   const unsigned rounds = ((unsigned)(n * units) + THREADS * U - 1) / (THREADS * U);
+   for(unsigned r = 0; r < rounds; ++r) {
+      mx::Half<T> h[U];
+      unsigned t[U], u[U];
+#pragma unroll
+      for(int k = 0; k < U; ++k, w.step()) {
+         t[k] = w.t;
+         u[k] = w.u;
+         const T* at = x + t[k] * row_stride + u[k] * mx::HALF;
+         if(t[k] >= (unsigned)n) h[k].zero();
+         else if(on_32) h[k].load(at);
+         else h[k].load_some(at, mx::HALF);
+      }
+#pragma unroll
+      for(int k = 0; k < U; ++k) {
+         uint32_t q[E::WORDS];
+         const uint32_t s = mx::encode_pair<MX8>(h[k], q);
+         const int row = t[k] < (unsigned)n ? rows[t[k]] : -1;
+         if(row < 0) continue;
+         mx::store_codes<E::WORDS>(p.codes + ((long long)row * units + u[k]) * (4 * E::WORDS), q);
+         if((u[k] & 1) == 0) p.scales[((long long)row * units + u[k]) / 2] = (uint8_t)s;
+      }
    }
+}
+
+template<class T, bool MX8>
+__global__ void __launch_bounds__(THREADS) read_kernel(T* __restrict__ out, long long row_stride, Pages p,
+                                                       const int32_t* __restrict__ cu, const int32_t* __restrict__ starts,
+                                                       long long tokens, int per, int units, bool on_32)
+{
+   using E = mx::Elem<MX8>;
+   __shared__ int rows[MAX_PER];
+   const long long t0 = (long long)blockIdx.x * per;
+   const int n = (int)min((long long)per, tokens - t0);
+   look_up(p, cu, starts, t0, n, rows);
+   out += t0 * row_stride;
+   Walk w(units);
+   while(w.t < (unsigned)n) {
+      uint32_t q[U][E::WORDS], s[U];
+      unsigned t[U], u[U];
+#pragma unroll
+      for(int k = 0; k < U; ++k, w.step()) {
+         t[k] = w.t;
+         u[k] = w.u;
+         const int row = t[k] < (unsigned)n ? rows[t[k]] : -1;
+#pragma unroll
+         for(int i = 0; i < E::WORDS; ++i) q[k][i] = 0;
+         s[k] = 0;
+         if(row >= 0) {
+            mx::load_codes<E::WORDS>(p.codes + ((long long)row * units + u[k]) * (4 * E::WORDS), q[k]);
+            s[k] = __ldg(p.scales + ((long long)row * units + u[k]) / 2);
+         }
+      }
+#pragma unroll
+      for(int k = 0; k < U; ++k) {
+         if(t[k] >= (unsigned)n) continue;
+         float v[mx::HALF];
+         mx::decode<MX8>(q[k], mx::scale_value(s[k]), v);
+         mx::Half<T> h;
+         h.set(v);
+         T* at = out + t[k] * row_stride + u[k] * mx::HALF;
+         if(on_32) h.store(at);
+         else h.store_some(at, mx::HALF);
+      }
+   }
+}
+
+// A CTA turns 128 positions x 64 channels around in shared memory: a lane
+// brings sixteen channels of a position, a group of lanes takes a channel's
+// positions out, 16 bytes each.  The tile is skewed by 8 words per 16
+// channels: the lanes of a warp, 8 positions x 4 groups of channels, store
+// into 32 banks.
+constexpr int RN = 128, RC = 64, RPITCH = RN + 4;
+template<class T, bool MX8>
+__global__ void __launch_bounds__(THREADS) read_channels_kernel(T* __restrict__ out, Pages p,
+                                                                const int32_t* __restrict__ starts,
+                                                                const int32_t* __restrict__ counts, long long n,
+                                                                int channels, unsigned tiles_n, unsigned tiles_c, bool on_16)
+{
+   using E = mx::Elem<MX8>;
+   constexpr int W = 16 / (int)sizeof(T);   // positions of a store
+   __shared__ int rows[RN];
+   __shared__ __align__(16) float tile[RC * RPITCH + 3 * 8];
+   const unsigned id = blockIdx.x, rest = id / tiles_n;
+   const int b = (int)(rest / tiles_c), c0 = (int)(rest % tiles_c) * RC;
+   const long long i0 = (long long)(id % tiles_n) * RN;
+   const long long count = min((long long)counts[b], n);
+   const bool any = i0 < count;
+   if(any) {
+      if(threadIdx.x < RN) {
+         const long long i = i0 + threadIdx.x;
+         rows[threadIdx.x] = i < count ? (int)p.slot(b, (long long)starts[b] + i) : -1;
+      }
+      __syncthreads();
+      uint32_t q[2][E::WORDS], s[2];
+#pragma unroll
+      for(int k = 0; k < 2; ++k) {
+         const int r = k * 64 + (threadIdx.x >> 2), c = c0 + (threadIdx.x & 3) * mx::HALF;
+         const int row = c < channels ? rows[r] : -1;
+#pragma unroll
+         for(int i = 0; i < E::WORDS; ++i) q[k][i] = 0;
+         s[k] = 0;
+         if(row >= 0) {
+            mx::load_codes<E::WORDS>(p.codes + ((long long)row * (channels / mx::HALF) + c / mx::HALF) * (4 * E::WORDS), q[k]);
+            s[k] = __ldg(p.scales + (long long)row * (channels / mx::BLOCK) + c / mx::BLOCK);
+         }
+      }
+#pragma unroll
+      for(int k = 0; k < 2; ++k) {
+         const int r = k * 64 + (threadIdx.x >> 2), g = threadIdx.x & 3;
+         float v[mx::HALF];
+         mx::decode<MX8>(q[k], mx::scale_value(s[k]), v);
+#pragma unroll
+         for(int i = 0; i < mx::HALF; ++i) tile[(g * mx::HALF + i) * RPITCH + g * 8 + r] = v[i];
+      }
+      __syncthreads();
+   }
+   for(int e = threadIdx.x; e < RC * (RN / W); e += THREADS) {
+      const int c = e / (RN / W), r = e % (RN / W) * W;
+      if(c0 + c >= channels || i0 + r >= n) continue;
+      float v[W];
+#pragma unroll
+      for(int i = 0; i < W / 4; ++i) {
+         const float4 f = any ? *reinterpret_cast<const float4*>(tile + c * RPITCH + (c >> 4) * 8 + r + 4 * i)
+                              : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+         v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w;
+      }
+      T* at = out + ((long long)b * channels + c0 + c) * n + i0 + r;
+      if(on_16 && i0 + r + W <= n) {
+         if constexpr(sizeof(T) == 4) *reinterpret_cast<float4*>(at) = make_float4(v[0], v[1], v[2], v[3]);
+         else *reinterpret_cast<uint4*>(at) = make_uint4(mx::pack2<T>(v[0], v[1]), mx::pack2<T>(v[2], v[3]),
+                                                         mx::pack2<T>(v[4], v[5]), mx::pack2<T>(v[6], v[7]));
+      } else {
+#pragma unroll
+         for(int i = 0; i < W; ++i)
+            if(i0 + r + i < n) at[i] = mx::from_f<T>(v[i]);
+      }
+   }
+}
+
+// tokens of a CTA: 32 K values, but two CTAs per SM before that
+int tokens_per_cta(const fufft_cache* c, long long tokens)
+{
+   int dev = 0, sms = 148;
+   if(cudaGetDevice(&dev) == cudaSuccess) sms = sm_count(dev);
+   long long per = std::max(1, 32768 / c->channels);
+   per = std::min<long long>(per, mx::ceil_div(tokens, 2 * sms));
+   return (int)std::min<long long>(per, MAX_PER);
 }
 
 template<class T>
@@ -108,10 +231,11 @@ fufft_status append(const fufft_cache* c, const void* x, long long row_stride, c
                     long long tokens, cudaStream_t st)
 {
    const T* xp = static_cast<const T*>(x);
-   const bool vec = aligned(x, 16) && (row_stride * (long long)sizeof(T)) % 16 == 0;
-   const unsigned grid = (unsigned)mx::ceil_div(tokens * (c->channels / 8), 256);
-   if(c->kind == FUFFT_CACHE_MX8) append_kernel<T, true><<<grid, 256, 0, st>>>(xp, row_stride, Pages(c), cu, starts, tokens, c->channels, vec);
-   else append_kernel<T, false><<<grid, 256, 0, st>>>(xp, row_stride, Pages(c), cu, starts, tokens, c->channels, vec);
+   const bool on_32 = aligned(x, 32) && row_stride * (long long)sizeof(T) % 32 == 0;
+   const int per = tokens_per_cta(c, tokens), units = c->channels / mx::HALF;
+   const unsigned grid = (unsigned)mx::ceil_div(tokens, per);
+   if(c->kind == FUFFT_CACHE_MX8) append_kernel<T, true><<<grid, THREADS, 0, st>>>(xp, row_stride, Pages(c), cu, starts, tokens, per, units, on_32);
+   else append_kernel<T, false><<<grid, THREADS, 0, st>>>(xp, row_stride, Pages(c), cu, starts, tokens, per, units, on_32);
    count_launch();
    return check(cudaGetLastError());
 }
@@ -121,10 +245,11 @@ fufft_status read(const fufft_cache* c, void* out, long long row_stride, const i
                   long long tokens, cudaStream_t st)
 {
    T* op = static_cast<T*>(out);
-   const bool vec = aligned(out, 16) && (row_stride * (long long)sizeof(T)) % 16 == 0;
-   const unsigned grid = (unsigned)mx::ceil_div(tokens * (c->channels / 8), 256);
-   if(c->kind == FUFFT_CACHE_MX8) read_kernel<T, true><<<grid, 256, 0, st>>>(op, row_stride, Pages(c), cu, starts, tokens, c->channels, vec);
-   else read_kernel<T, false><<<grid, 256, 0, st>>>(op, row_stride, Pages(c), cu, starts, tokens, c->channels, vec);
+   const bool on_32 = aligned(out, 32) && row_stride * (long long)sizeof(T) % 32 == 0;
+   const int per = tokens_per_cta(c, tokens), units = c->channels / mx::HALF;
+   const unsigned grid = (unsigned)mx::ceil_div(tokens, per);
+   if(c->kind == FUFFT_CACHE_MX8) read_kernel<T, true><<<grid, THREADS, 0, st>>>(op, row_stride, Pages(c), cu, starts, tokens, per, units, on_32);
+   else read_kernel<T, false><<<grid, THREADS, 0, st>>>(op, row_stride, Pages(c), cu, starts, tokens, per, units, on_32);
    count_launch();
    return check(cudaGetLastError());
 }
@@ -134,9 +259,11 @@ fufft_status read_channels(const fufft_cache* c, void* out, long long n, const i
                            cudaStream_t st)
 {
    T* op = static_cast<T*>(out);
-   const unsigned grid = (unsigned)(mx::ceil_div(n, RT) * mx::ceil_div(c->channels, RT) * c->batch);
-   if(c->kind == FUFFT_CACHE_MX8) read_channels_kernel<T, true><<<grid, 256, 0, st>>>(op, Pages(c), starts, counts, n, c->channels);
-   else read_channels_kernel<T, false><<<grid, 256, 0, st>>>(op, Pages(c), starts, counts, n, c->channels);
+   const unsigned tn = (unsigned)mx::ceil_div(n, RN), tc = (unsigned)mx::ceil_div(c->channels, RC);
+   const unsigned grid = tn * tc * (unsigned)c->batch;
+   const bool on_16 = aligned(out, 16) && n * (long long)sizeof(T) % 16 == 0;
+   if(c->kind == FUFFT_CACHE_MX8) read_channels_kernel<T, true><<<grid, THREADS, 0, st>>>(op, Pages(c), starts, counts, n, c->channels, tn, tc, on_16);
+   else read_channels_kernel<T, false><<<grid, THREADS, 0, st>>>(op, Pages(c), starts, counts, n, c->channels, tn, tc, on_16);
    count_launch();
    return check(cudaGetLastError());
 }
@@ -212,7 +339,7 @@ fufft_status fufft_cache_read_channels(const fufft_cache* c, void* out, fufft_dt
    if(bad_dtype(dtype)) return FUFFT_ERR_INVALID_ARG;
    if(n < 0 || n > cache::MAX_TOKENS) return FUFFT_ERR_INVALID_SIZE;
    if(n == 0 || c->batch == 0) return FUFFT_OK;
-   if(mx::ceil_div(n, cache::RT) * mx::ceil_div(c->channels, cache::RT) > 0x7fffffffll / c->batch) return FUFFT_ERR_INVALID_SIZE;
+   if(mx::ceil_div(n, cache::RN) * mx::ceil_div(c->channels, cache::RC) > 0x7fffffffll / c->batch) return FUFFT_ERR_INVALID_SIZE;
    if(!out || !starts || !counts) return FUFFT_ERR_INVALID_ARG;
    if(!aligned(out, dtype_align(dtype)) || !aligned(starts, 4) || !aligned(counts, 4)) return FUFFT_ERR_MISALIGNED;
    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);

@@ -35,26 +35,6 @@ struct Pages {
       const int page = table[b * table_stride + k];
       return page < 0 || page >= pages ? -1 : (long long)page * page_size + (pos - k * page_size);
    }
-
-   // eight values of row `slot` from channel c (a multiple of 8)
-   template<bool MX8> __device__ __forceinline__ void load8(long long slot, int c, int channels, float* v) const
-   {
-      using E = mx::Elem<MX8>;
-      uint32_t w[E::WORDS];
-      const uint32_t* at = reinterpret_cast<const uint32_t*>(codes + slot * (long long)(channels / 8) * (4 * E::WORDS)) +
-                           (c / 8) * E::WORDS;
-      if constexpr(MX8) {
-         const uint2 q = *reinterpret_cast<const uint2*>(at);
-         w[0] = q.x;
-         w[1] = q.y;
-      } else {
-         w[0] = *at;
-      }
-      const float s = mx::scale_value(scales[slot * (channels / mx::BLOCK) + c / mx::BLOCK]);
-      E::decode8(w, v);
-#pragma unroll
-      for(int i = 0; i < 8; ++i) v[i] *= s;
-   }
 };
 
 fufft_status check_cache(const fufft_cache* c);

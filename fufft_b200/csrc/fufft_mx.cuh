@@ -81,49 +81,122 @@ template<> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w)
    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 
-// eight consecutive values; vec: p is 16-byte aligned and all eight exist
-template<class T> __device__ __forceinline__ void load8(const T* p, bool vec, int count, float* v)
+// 32-byte transfers (p 32-byte aligned)
+__device__ __forceinline__ void load32(const void* p, uint32_t* w)
 {
-   if(vec) {
-      if constexpr(sizeof(T) == 4) {
-         const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-         v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-         v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-      } else {
-         const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
-         const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-         for(int i = 0; i < 4; ++i) {
-            const float2 f = unpack2<T>(w[i]);
-            v[2 * i] = f.x;
-            v[2 * i + 1] = f.y;
-         }
-      }
-      return;
-   }
-#pragma unroll
-   for(int i = 0; i < 8; ++i) v[i] = i < count ? to_f(p[i]) : 0.0f;
+   asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(p));
 }
-template<class T> __device__ __forceinline__ void store8(T* p, bool vec, int count, const float* v)
+__device__ __forceinline__ void store32(void* p, const uint32_t* w)
 {
-   if(vec) {
-      if constexpr(sizeof(T) == 4) {
-         reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-         reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-      } else {
-         *reinterpret_cast<uint4*>(p) = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]),
-                                                   pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
-      }
-      return;
-   }
-#pragma unroll
-   for(int i = 0; i < 8; ++i)
-      if(i < count) p[i] = from_f<T>(v[i]);
+   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                :: "l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
 }
 
 // |x| as bits: they order like the values, an infinity above every number and
 // a NaN above an infinity, so an integer maximum keeps both
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// maximum of abs_bits over N values as they lie in memory, three words an
+// instruction; of 16-bit values two maxima, in the halves of a word
+template<class T, int N> __device__ __forceinline__ uint32_t max_words(const uint32_t* w)
+{
+   constexpr uint32_t MASK = sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu;
+   uint32_t m = w[0] & MASK;
+#pragma unroll
+   for(int i = 1; i + 1 < N; i += 2) {
+      if constexpr(sizeof(T) == 4) m = __vimax3_u32(m, w[i] & MASK, w[i + 1] & MASK);
+      else m = __vimax3_u16x2(m, w[i] & MASK, w[i + 1] & MASK);
+   }
+   if constexpr(sizeof(T) == 4) return max(m, w[N - 1] & MASK);
+   else return __vimax3_u16x2(m, m, w[N - 1] & MASK);
+}
+// values v[2 i], v[2 i + 1] = those of w[i] times a power of two
+template<class T> __device__ __forceinline__ void scaled_pair(uint32_t w, float factor, float* v)
+{
+   const float2 f = fmul2(unpack2<T>(w), make_float2(factor, factor));
+   v[0] = f.x;
+   v[1] = f.y;
+}
+
+// Sixteen consecutive values as they lie in memory: half a block, the unit of
+// the format kernels (two neighbouring lanes a block).
+constexpr int HALF = 16;
+template<class T> struct Half {
+   static constexpr int WORDS = HALF * (int)sizeof(T) / 4;
+   uint32_t w[WORDS];
+   // all sixteen, p on 32 bytes
+   __device__ __forceinline__ void load(const T* p)
+   {
+#pragma unroll
+      for(int i = 0; i < WORDS / 8; ++i) load32(reinterpret_cast<const uint8_t*>(p) + 32 * i, w + 8 * i);
+   }
+   __device__ __forceinline__ void store(T* p) const
+   {
+#pragma unroll
+      for(int i = 0; i < WORDS / 8; ++i) store32(reinterpret_cast<uint8_t*>(p) + 32 * i, w + 8 * i);
+   }
+   // the first `count`, anywhere; zeros after them
+   __device__ __forceinline__ void load_some(const T* p, int count)
+   {
+#pragma unroll
+      for(int i = 0; i < WORDS; ++i) {
+         if constexpr(sizeof(T) == 4) {
+            w[i] = i < count ? __float_as_uint(p[i]) : 0u;
+         } else {
+            const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
+            w[i] = (2 * i < count ? (uint32_t)q[2 * i] : 0u) | (2 * i + 1 < count ? (uint32_t)q[2 * i + 1] << 16 : 0u);
+         }
+      }
+   }
+   __device__ __forceinline__ void store_some(T* p, int count) const
+   {
+#pragma unroll
+      for(int i = 0; i < WORDS; ++i) {
+         if constexpr(sizeof(T) == 4) {
+            if(i < count) p[i] = __uint_as_float(w[i]);
+         } else {
+            uint16_t* q = reinterpret_cast<uint16_t*>(p);
+            if(2 * i < count) q[2 * i] = (uint16_t)w[i];
+            if(2 * i + 1 < count) q[2 * i + 1] = (uint16_t)(w[i] >> 16);
+         }
+      }
+   }
+   __device__ __forceinline__ void zero()
+   {
+#pragma unroll
+      for(int i = 0; i < WORDS; ++i) w[i] = 0;
+   }
+   // maximum of abs_bits
+   __device__ __forceinline__ uint32_t max_bits() const
+   {
+      const uint32_t m = max_words<T, WORDS>(w);
+      if constexpr(sizeof(T) == 4) return m;
+      else return abs_bits(unpack2<T>(max(m >> 16, m & 0xffffu)).x);
+   }
+   // the values times a power of two
+   __device__ __forceinline__ void scaled(float factor, float* v) const
+   {
+#pragma unroll
+      for(int i = 0; i < HALF / 2; ++i) {
+         if constexpr(sizeof(T) == 4) {
+            const float2 f = fmul2(make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1])), make_float2(factor, factor));
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+         } else {
+            scaled_pair<T>(w[i], factor, v + 2 * i);
+         }
+      }
+   }
+   __device__ __forceinline__ void set(const float* v)
+   {
+#pragma unroll
+      for(int i = 0; i < WORDS; ++i) {
+         if constexpr(sizeof(T) == 4) w[i] = __float_as_uint(v[i]);
+         else w[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+      }
+   }
+};
 
 // scale byte of a block from the maximum of abs_bits
 template<int EMAX> __device__ __forceinline__ uint32_t scale_byte(uint32_t max_bits)
@@ -173,54 +246,79 @@ __device__ __forceinline__ void e4m3_decode4(uint32_t c, uint32_t* h)
 }
 __device__ __forceinline__ float2 half2_f(uint32_t h) { return __half22float2(*reinterpret_cast<const __half2*>(&h)); }
 
-// the two formats a cache stores; eight codes are CODE_BYTES bytes in CODE_WORDS words
+// the two element formats; sixteen codes are WORDS words
 template<bool MX8> struct Elem;
 template<> struct Elem<false> {
-   static constexpr int EMAX = 2, WORDS = 1;
-   __device__ static __forceinline__ void encode8(const float* v, uint32_t* w) { w[0] = e2m1_encode8(v); }
-   __device__ static __forceinline__ void decode8(const uint32_t* w, float* v)
+   static constexpr int EMAX = 2, WORDS = 2;
+   __device__ static __forceinline__ void encode(const float* v, uint32_t* w)
    {
-      uint32_t h[4];
+      w[0] = e2m1_encode8(v);
+      w[1] = e2m1_encode8(v + 8);
+   }
+   __device__ static __forceinline__ void halves(const uint32_t* w, uint32_t* h)
+   {
       e2m1_decode8(w[0], h);
-#pragma unroll
-      for(int i = 0; i < 4; ++i) {
-         const float2 f = half2_f(h[i]);
-         v[2 * i] = f.x;
-         v[2 * i + 1] = f.y;
-      }
+      e2m1_decode8(w[1], h + 4);
    }
 };
 template<> struct Elem<true> {
-   static constexpr int EMAX = 8, WORDS = 2;
-   __device__ static __forceinline__ void encode8(const float* v, uint32_t* w)
+   static constexpr int EMAX = 8, WORDS = 4;
+   __device__ static __forceinline__ void encode(const float* v, uint32_t* w)
    {
-      w[0] = e4m3_encode4(v);
-      w[1] = e4m3_encode4(v + 4);
-   }
-   __device__ static __forceinline__ void decode8(const uint32_t* w, float* v)
-   {
-      uint32_t h[4];
-      e4m3_decode4(w[0], h);
-      e4m3_decode4(w[1], h + 2);
 #pragma unroll
-      for(int i = 0; i < 4; ++i) {
-         const float2 f = half2_f(h[i]);
-         v[2 * i] = f.x;
-         v[2 * i + 1] = f.y;
-      }
+      for(int i = 0; i < 4; ++i) w[i] = e4m3_encode4(v + 4 * i);
+   }
+   __device__ static __forceinline__ void halves(const uint32_t* w, uint32_t* h)
+   {
+#pragma unroll
+      for(int i = 0; i < 4; ++i) e4m3_decode4(w[i], h + 2 * i);
    }
 };
-
-// block of 32 spread over four neighbouring lanes, eight values each: the
-// block's scale byte, in all four
-template<int EMAX> __device__ __forceinline__ uint32_t block_scale4(const float* v)
+// sixteen codes -> values times `scale`
+template<bool MX8> __device__ __forceinline__ void decode(const uint32_t* w, float scale, float* v)
 {
-   uint32_t m = 0;
+   uint32_t h[8];
+   Elem<MX8>::halves(w, h);
 #pragma unroll
-   for(int i = 0; i < 8; ++i) m = max(m, abs_bits(v[i]));
+   for(int i = 0; i < 8; ++i) {
+      const float2 f = fmul2(half2_f(h[i]), make_float2(scale, scale));
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+   }
+}
+// 8 (MX4) or 16 (MX8) bytes of codes
+template<int WORDS> __device__ __forceinline__ void load_codes(const uint8_t* p, uint32_t* w)
+{
+   if constexpr(WORDS == 4) {
+      const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
+      w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
+   } else {
+      const uint2 q = __ldg(reinterpret_cast<const uint2*>(p));
+      w[0] = q.x; w[1] = q.y;
+   }
+}
+template<int WORDS> __device__ __forceinline__ void store_codes(uint8_t* p, const uint32_t* w)
+{
+   if constexpr(WORDS == 4) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+   else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+}
+
+// A block in two neighbouring lanes, sixteen values each (all 32 lanes take
+// part): its scale byte, and the lane's codes.
+template<bool MX8, class T> __device__ __forceinline__ uint32_t encode_pair(const Half<T>& h, uint32_t* w)
+{
+   uint32_t m = h.max_bits();
    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-   m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-   return scale_byte<EMAX>(m);
+   const uint32_t s = scale_byte<Elem<MX8>::EMAX>(m);
+   const float inv = scale_inverse(s);
+   float v[HALF];
+   h.scaled(inv, v);
+   if(s == 255u) {   // zero codes under a NaN scale
+#pragma unroll
+      for(int i = 0; i < HALF; ++i) v[i] = 0.0f;
+   }
+   Elem<MX8>::encode(v, w);
+   return s;
 }
 
 }  // namespace mx
