@@ -55,7 +55,7 @@ __device__ __forceinline__ void look_up(const Pages& p, const int32_t* cu, const
    if(threadIdx.x < n) {
       const long long t = t0 + threadIdx.x;
       const int b = find_sequence(cu, p.batch, t);
-      rows[threadIdx.x] = b < 0 ? -1 : (int)p.slot(b, (long long)starts[b] + (t - cu[b]));
+      rows[threadIdx.x] = b < 0 ? -1 : p.slot(b, (long long)starts[b] + (t - cu[b]));
    }
    __syncthreads();
 }
@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(THREADS) read_channels_kernel(T* __restrict__ 
    if(any) {
       if(threadIdx.x < RN) {
          const long long i = i0 + threadIdx.x;
-         rows[threadIdx.x] = i < count ? (int)p.slot(b, (long long)starts[b] + i) : -1;
+         rows[threadIdx.x] = i < count ? p.slot(b, (long long)starts[b] + i) : -1;
       }
       __syncthreads();
       uint32_t q[2][E::WORDS], s[2];

@@ -26,14 +26,15 @@ struct Pages {
    }
 
    // row of the flattened pages that holds position pos of sequence b, or -1
-   // where the sequence has no page there
-   __device__ __forceinline__ long long slot(int b, long long pos) const
+   // where the sequence has no page there.  Lengths are 32 bits, so positions
+   // beyond them hold nothing; pages * page_size stays below 2^31.
+   __device__ __forceinline__ int slot(int b, long long pos) const
    {
-      if(pos < 0) return -1;
-      const long long k = pos / page_size;
-      if(k >= max_pages) return -1;
-      const int page = table[b * table_stride + k];
-      return page < 0 || page >= pages ? -1 : (long long)page * page_size + (pos - k * page_size);
+      if(pos < 0 || pos > 0x7fffffffll) return -1;
+      const unsigned k = (unsigned)pos / (unsigned)page_size;
+      if(k >= (unsigned)max_pages) return -1;
+      const int page = __ldg(table + b * table_stride + k);
+      return page < 0 || page >= pages ? -1 : page * page_size + (int)((unsigned)pos - k * (unsigned)page_size);
    }
 };
 

@@ -16,6 +16,7 @@ namespace cache {
 constexpr int CH = 16;        // channels per thread: one 8-byte (MX4) or 16-byte (MX8) load a token
 constexpr int TILE = 256;     // lags whose cache rows are looked up together, at most
 constexpr int THREADS = 256;
+constexpr int MAX_SPLIT = 8;    // CTAs of a portable cluster
 
 struct ConvStep {
    const int32_t* lengths;
@@ -113,6 +114,53 @@ __device__ __forceinline__ void finish(const ConvStep& a, int b, int c, float y)
    else finish<__nv_bfloat16>(a, b, c, y);
 }
 
+// a thread's sums, to [sequence][slot][lanes x 16] in shared memory
+template<int NB>
+__device__ __forceinline__ void park(float* joined, const float2 (&acc)[NB][CH / 2], int slot, int lane, int slots, int lanes)
+{
+#pragma unroll
+   for(int s = 0; s < NB; ++s)
+#pragma unroll
+      for(int i = 0; i < CH / 4; ++i)
+         *reinterpret_cast<float4*>(joined + ((s * slots + slot) * lanes + lane) * CH + 4 * i) =
+            make_float4(acc[s][2 * i].x, acc[s][2 * i].y, acc[s][2 * i + 1].x, acc[s][2 * i + 1].y);
+}
+
+// Adds the slots of this CTA in their order, then the CTAs of its cluster in
+// theirs (through distributed shared memory, a part of the results each), and
+// writes the results, or the cluster's part of them where there are several.
+template<int NB>
+__device__ __forceinline__ void join(float* joined, const ConvStep& a, const Pages& p, int width, int slots, int threads,
+                                     int rank, int b0, int c0)
+{
+   __syncthreads();
+   for(int e = threadIdx.x; e < NB * width; e += threads) {
+      float* at = joined + e / width * (slots * width) + e % width;
+      float y = *at;
+      for(int k = 1; k < slots; ++k) y += at[k * width];
+      *at = y;
+   }
+   if(a.split > 1) tc::cluster_sync();
+   else __syncthreads();
+   for(int e = threadIdx.x + rank * threads; e < NB * width; e += threads * a.split) {
+      const int s = e / width, i = e % width;
+      if(b0 + s >= p.batch || c0 + i >= a.channels) continue;
+      const float* at = joined + s * (slots * width) + i;
+      float y = *at;
+      if(a.split > 1) {
+         float v[MAX_SPLIT];
+#pragma unroll
+         for(int r = 0; r < MAX_SPLIT; ++r) v[r] = r < a.split ? tc::load_peer(tc::peer_smem(at, r)) : 0.0f;
+         y = 0.0f;
+#pragma unroll
+         for(int r = 0; r < MAX_SPLIT; ++r) y += v[r];
+      }
+      if(a.partial) a.partial[((long long)(blockIdx.x / a.split) * p.batch + b0 + s) * a.channels + c0 + i] = y;
+      else finish(a, b0 + s, c0 + i, y);
+   }
+   if(a.split > 1) tc::cluster_sync();   // nobody leaves while its sums are being read
+}
+
 // A CTA: a.lanes x 16 channels of NB sequences, a.slots lags at a time; the
 // same taps serve the NB sequences, which stand at different positions of
 // their pages but at the same lag.  Per stored value: half a conversion, one
@@ -154,7 +202,7 @@ __global__ void __launch_bounds__(THREADS, 2) conv_step_kernel(Pages p, ConvStep
       __syncthreads();
       for(int e = threadIdx.x; e < count; e += THREADS)
 #pragma unroll
-         for(int s = 0; s < NB; ++s) rows[s][e] = len[s] > j0 + e ? (int)p.slot(b0 + s, len[s] - 1 - (j0 + e)) : -1;
+         for(int s = 0; s < NB; ++s) rows[s][e] = len[s] > j0 + e ? p.slot(b0 + s, len[s] - 1 - (j0 + e)) : -1;
       __syncthreads();
       if(!active) continue;
       for(int j = slot; j < count; j += a.slots * U) {
@@ -190,38 +238,8 @@ __global__ void __launch_bounds__(THREADS, 2) conv_step_kernel(Pages p, ConvStep
       }
    }
 
-   // the slots of this CTA, in their order
-   const int width = a.lanes * CH, pitch = a.slots * width;
-#pragma unroll
-   for(int s = 0; s < NB; ++s)
-      if(slot < a.slots)
-#pragma unroll
-         for(int i = 0; i < CH / 4; ++i)
-            *reinterpret_cast<float4*>(joined + s * pitch + (slot * a.lanes + lane) * CH + 4 * i) =
-               make_float4(acc[s][2 * i].x, acc[s][2 * i].y, acc[s][2 * i + 1].x, acc[s][2 * i + 1].y);
-   __syncthreads();
-   for(int e = threadIdx.x; e < NB * width; e += THREADS) {
-      float* at = joined + e / width * pitch + e % width;
-      float y = *at;
-      for(int k = 1; k < a.slots; ++k) y += at[k * width];
-      *at = y;
-   }
-   // the CTAs of the cluster, in their order
-   if(a.split > 1) tc::cluster_sync();
-   else __syncthreads();
-   for(int e = threadIdx.x + rank * THREADS; e < NB * width; e += THREADS * a.split) {
-      const int s = e / width, i = e % width;
-      if(b0 + s >= p.batch || c0 + i >= a.channels) continue;
-      const float* at = joined + s * pitch + i;
-      float y = *at;
-      if(a.split > 1) {
-         y = 0.0f;
-         for(int r = 0; r < a.split; ++r) y += tc::load_peer(tc::peer_smem(at, r));
-      }
-      if(a.partial) a.partial[((long long)(worker / a.split) * p.batch + b0 + s) * a.channels + c0 + i] = y;
-      else finish(a, b0 + s, c0 + i, y);
-   }
-   if(a.split > 1) tc::cluster_sync();   // nobody leaves while its sums are being read
+   if(slot < a.slots) park<NB>(joined, acc, slot, lane, a.slots, a.lanes);
+   join<NB>(joined, a, p, a.lanes * CH, a.slots, THREADS, rank, b0, c0);
 }
 
 // joins the clusters in their order
@@ -233,6 +251,489 @@ __global__ void __launch_bounds__(256) conv_join_kernel(ConvStep a, int batch)
    for(int k = 0; k < a.outer; ++k) y += a.partial[(long long)k * batch * a.channels + g];
    finish(a, (int)(g / a.channels), (int)(g % a.channels), y);
 }
+
+// ---------------------------------------------------------------------------
+// The same through a ring of stages in shared memory, where rows are long
+// enough to be copied one by one: what bounds the step is then reading the
+// cache, with three instructions a value left to issue meanwhile.  A stage is
+// `lags` lags of NS sequences: their rows of codes (tensor copies that gather
+// four rows each; a row that is not there is one outside the tensor, and reads
+// as zeros), the taps (one tensor copy, 16-byte chunks permuted so that the
+// lanes' wide loads fall on different banks) and the scales, with the taps that
+// heads share.  A warp fills each slot of the ring.  Eight warps sum: a thread keeps 16
+// channels of the NS sequences, so a tap is widened once for all of them.
+//
+// Two ways to sum a value.  Where every scale of the stage is a half-precision
+// number (2^-24 .. 2^15) and every row is there, an exact fma widens the half
+// x and scales it, one instruction on both halves of the FMA pipe, and half a
+// packed fma adds it times its tap: twice as fast as the general way, whose
+// widening and packed product and sum all go to one half of the pipe (B200, a
+// loop of them alone: 29 values a clock and SM).
+// ---------------------------------------------------------------------------
+namespace pipe {
+constexpr int CONSUMERS = 8, PRODUCERS = 4, THREADS = (CONSUMERS + PRODUCERS) * 32;   // warps that sum; that fill
+constexpr int MAX_PAIRS = 256;                                                         // rows of a stage
+constexpr int MAX_STAGES = PRODUCERS;
+
+struct Args {
+   ConvStep a;
+   unsigned int* status;
+   int lags, stages, stage_bytes, codes_at, scales_at;   // of a stage: lags; offsets of its parts (taps at 0)
+   int row_bytes;                                        // of the CTA's chunk
+   int tap_bytes;                                        // of a lag's taps in the chunk
+   bool quads;                                           // four blocks' scales at once
+};
+
+__device__ __forceinline__ void arrive(uint64_t* bar)
+{
+   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void load_taps(const CUtensorMap* tm, void* dst, int x, int y, int z, uint64_t* bar)
+{
+   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                :: "r"(smem_u32(dst)), "l"(tm), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar)) : "memory");
+}
+// four rows of a 2-D map whose box is one row high, side by side; x a multiple of 16 bytes
+__device__ __forceinline__ void gather4(const CUtensorMap* tm, void* dst, int x, int4 r, uint64_t* bar)
+{
+   asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
+                :: "r"(smem_u32(dst)), "l"(tm), "r"(x), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w), "r"(smem_u32(bar)) : "memory");
+}
+// x times scale, halves widened: exact
+__device__ __forceinline__ float2 widen_scaled(uint32_t x, uint32_t scale)
+{
+   float2 r;
+   asm("{\n\t.reg .b16 a, b, c, d;\n\tmov.b32 {a, b}, %2;\n\tmov.b32 {c, d}, %3;\n\t"
+       "fma.rn.f32.f16 %0, a, c, %4;\n\tfma.rn.f32.f16 %1, b, c, %4;\n\t}"
+       : "=f"(r.x), "=f"(r.y) : "r"(x), "r"(scale), "f"(0.0f));
+   return r;
+}
+
+// A scale as a stage holds it: the half-precision number in the low half, its byte in bits 16 .. 23.
+constexpr uint32_t NO_HALF = 1u << 31, NO_ROW = 1u << 30;
+__device__ __forceinline__ uint32_t scale_entry(uint32_t s)
+{
+   const int e = (int)s - 127;
+   const uint32_t half = e > 15 || e < -24 ? 0u : e >= -14 ? (uint32_t)(e + 15) << 10 : 1u << (e + 24);
+   return half | s << 16 | (half ? 0u : NO_HALF);
+}
+
+// cache rows of the pairs (lag, sequence) of a stage, pair = lag * NS + sequence; -1 without one
+template<int NS>
+__device__ __forceinline__ void find_rows(const Pages& p, int b0, int len, int lane, int pairs, int filled, long long j0, int* rows)
+{
+   __syncwarp();
+   for(int pair = lane; pair < filled; pair += 32) {   // a lane's sequence, lane % NS, is the same throughout
+      const long long j = j0 + pair / NS;
+      rows[pair] = pair < pairs && j < len ? p.slot(b0 + lane % NS, (long long)len - 1 - j) : -1;
+   }
+   __syncwarp();
+}
+
+// The scales of a stage, [pair][block]: a lane takes W blocks of a row, eight
+// rows a batch.  The first batch is loaded before the stage is known to be
+// free, and put there when it is.
+template<int W> struct Scales {
+   static constexpr int BATCH = 8;
+   int each, at_once, mine, b0;   // 2^each lanes a row, rows at a time, this lane's row and its first block
+   uint32_t raw[BATCH];
+   int row[BATCH];
+   __device__ __forceinline__ Scales(int blocks, int lane)
+   {
+      const int across = blocks / W;
+      each = across <= 1 ? 0 : min(5, 32 - __clz(across - 1));
+      at_once = 32 >> each;
+      mine = lane >> each;
+      b0 = (lane & ((1 << each) - 1)) * W;
+   }
+   __device__ __forceinline__ void load(const int* rows, const uint8_t* scales, int row_scales, int first, int b, int blocks, int pairs)
+   {
+#pragma unroll
+      for(int k = 0; k < BATCH; ++k) {
+         const int pair = first + k * at_once + mine;
+         row[k] = pair < pairs && b < blocks ? rows[pair] : -2;
+         if(row[k] >= 0) {
+            const uint8_t* at = scales + (long long)row[k] * row_scales + b;
+            if constexpr(W == 4) raw[k] = __ldg(reinterpret_cast<const unsigned int*>(at));
+            else raw[k] = __ldg(at);
+         }
+      }
+   }
+   // the entries' flags
+   __device__ __forceinline__ uint32_t store(const uint32_t* entry, uint32_t* out, int first, int b, int blocks) const
+   {
+      uint32_t seen = 0;
+#pragma unroll
+      for(int k = 0; k < BATCH; ++k) {
+         if(row[k] == -2) continue;
+         uint32_t* to = out + (first + k * at_once + mine) * blocks + b;
+         if constexpr(W == 4) {
+            uint4 e = make_uint4(NO_ROW, NO_ROW, NO_ROW, NO_ROW);
+            if(row[k] >= 0) e = make_uint4(entry[raw[k] & 255], entry[raw[k] >> 8 & 255], entry[raw[k] >> 16 & 255], entry[raw[k] >> 24]);
+            seen |= e.x | e.y | e.z | e.w;
+            *reinterpret_cast<uint4*>(to) = e;
+         } else {
+            const uint32_t e = row[k] >= 0 ? entry[raw[k]] : NO_ROW;
+            seen |= e;
+            *to = e;
+         }
+      }
+      return seen;
+   }
+   // what the first batch has left
+   __device__ __forceinline__ uint32_t rest(const int* rows, const uint32_t* entry, const uint8_t* scales, int row_scales, uint32_t* out,
+                                            int blocks, int pairs)
+   {
+      uint32_t seen = 0;
+      for(int base = 0; base < blocks; base += W << each)
+         for(int first = base ? 0 : BATCH * at_once; first < pairs; first += BATCH * at_once) {
+            load(rows, scales, row_scales, first, base + b0, blocks, pairs);
+            seen |= store(entry, out, first, base + b0, blocks);
+         }
+      return seen;
+   }
+};
+
+// The taps of a stage that blocks share, [lag][block], as numbers; eight loads under way.
+template<class TT>
+__device__ __forceinline__ void stage_taps(const TT* taps, long long stride, int c0, int group, float* out, int pitch, int blocks,
+                                           int lags, int lane)
+{
+   const int each = blocks <= 1 ? 0 : min(5, 32 - __clz(blocks - 1)), at_once = 32 >> each, mine = lane >> each;
+   for(int b = lane & ((1 << each) - 1); b < blocks; b += 1 << each) {
+      const int head = (c0 + b * mx::BLOCK) / group;
+      for(int first = mine; first < lags; first += 8 * at_once) {
+         TT t[8];
+#pragma unroll
+         for(int k = 0; k < 8; ++k)
+            if(first + k * at_once < lags) t[k] = taps[(first + k * at_once) * stride + head];
+#pragma unroll
+         for(int k = 0; k < 8; ++k)
+            if(first + k * at_once < lags) out[(first + k * at_once) * pitch + b] = mx::to_f(t[k]);
+      }
+   }
+}
+
+// What a consumer does with its lags of a stage.  FAST: every scale a half, every row there.
+template<bool MX8, class TT, bool HEAD, int NB> struct Lag {   // what a thread reads of one lag
+   uint32_t q[NB][MX8 ? 4 : 2], e[NB], t[HEAD ? 1 : CH * sizeof(TT) / 4];
+   __device__ __forceinline__ void load(const uint8_t* at, uint32_t off, const uint8_t* codes, int row, const uint32_t* scales, int blocks)
+   {
+#pragma unroll
+      for(int s = 0; s < NB; ++s) {
+         e[s] = scales[s * blocks];
+         if constexpr(MX8) {
+            const uint4 x = *reinterpret_cast<const uint4*>(codes + s * row);
+            q[s][0] = x.x; q[s][1] = x.y; q[s][2] = x.z; q[s][3] = x.w;
+         } else {
+            const uint2 x = *reinterpret_cast<const uint2*>(codes + s * row);
+            q[s][0] = x.x; q[s][1] = x.y;
+         }
+      }
+      if constexpr(HEAD) {
+         t[0] = *reinterpret_cast<const uint32_t*>(at + off);
+      } else {
+         const uint32_t flip = (off >> 3) & 0x70;
+#pragma unroll
+         for(int k = 0; k < (int)(CH * sizeof(TT) / 16); ++k) {
+            const uint4 x = *reinterpret_cast<const uint4*>(at + ((off + 16 * k) ^ flip));
+            t[4 * k] = x.x; t[4 * k + 1] = x.y; t[4 * k + 2] = x.z; t[4 * k + 3] = x.w;
+         }
+      }
+   }
+   __device__ __forceinline__ float2 tap(int k) const
+   {
+      if constexpr(HEAD) return make_float2(__uint_as_float(t[0]), __uint_as_float(t[0]));
+      else if constexpr(sizeof(TT) == 4) return make_float2(__uint_as_float(t[2 * k]), __uint_as_float(t[2 * k + 1]));
+      else return mx::unpack2<__nv_bfloat16>(t[k]);
+   }
+   template<bool FAST> __device__ __forceinline__ void sum(float2 (&acc)[NB][CH / 2]) const
+   {
+      float2 w[HEAD ? 1 : CH / 2];
+#pragma unroll
+      for(int k = 0; k < (HEAD ? 1 : CH / 2); ++k) w[k] = tap(k);
+#pragma unroll
+      for(int s = 0; s < NB; ++s) {
+         uint32_t v[CH / 2];
+         mx::Elem<MX8>::halves(q[s], v);
+         if constexpr(FAST) {
+#pragma unroll
+            for(int k = 0; k < CH / 2; ++k) acc[s][k] = ffma2(widen_scaled(v[k], e[s]), w[HEAD ? 0 : k], acc[s][k]);
+         } else {
+            if(e[s] & NO_ROW) continue;
+            const float scale = mx::scale_value(e[s] >> 16 & 255);
+#pragma unroll
+            for(int k = 0; k < CH / 2; ++k) acc[s][k] = ffma2(fmul2(mx::half2_f(v[k]), make_float2(scale, scale)), w[HEAD ? 0 : k], acc[s][k]);
+         }
+      }
+   }
+};
+// Where a thread's first lag lies in a stage, and its steps from lag to lag.
+struct Path {
+   uint32_t tap, tap_step;
+   int codes, codes_step, row, scales, scales_step, blocks, slot, slots;
+};
+template<bool MX8, class TT, bool HEAD, int NB, bool FAST>
+__device__ __forceinline__ void sum_stage(const uint8_t* at, const Path& w, int count, float2 (&acc)[NB][CH / 2])
+{
+   using L = Lag<MX8, TT, HEAD, NB>;
+   uint32_t tap = w.tap;
+   const uint8_t* codes = at + w.codes;
+   const uint32_t* scales = reinterpret_cast<const uint32_t*>(at + w.scales);
+#pragma unroll 1
+   for(int l = w.slot; l < count; l += w.slots, tap += w.tap_step, codes += w.codes_step, scales += w.scales_step) {
+      L one;
+      one.load(at, tap, codes, w.row, scales, w.blocks);
+      one.template sum<FAST>(acc);
+   }
+}
+
+template<class TT, bool HEAD, int NS, int W>
+__device__ __forceinline__ void fill(const CUtensorMap* codes_map, const CUtensorMap* taps_map, const Pages& p, const Args& g, uint8_t* ring,
+                                     uint64_t* full, uint64_t* empty, uint32_t* flags, const uint32_t* entry, int* found, int st, int n,
+                                     int worker, int workers, int longest, int mine, int b0, int c0, int x, int blocks, int lane)
+{
+   const ConvStep& a = g.a;
+   uint8_t* at = ring + st * g.stage_bytes;
+   uint32_t* out = reinterpret_cast<uint32_t*>(at + g.scales_at);
+   const uint8_t* scales = p.scales + c0 / mx::BLOCK;
+   const int row_scales = a.channels / mx::BLOCK;
+   Scales<W> sc(blocks, lane);
+   uint32_t phase = 1;
+   bool ok = true;
+   for(int i = st; i < n; i += g.stages, phase ^= 1) {
+      const long long j0 = (long long)(worker + (long long)i * workers) * g.lags;
+      const int count = (int)min((long long)g.lags, longest - j0);
+      find_rows<NS>(p, b0, mine, lane, count * NS, g.lags * NS, j0, found);
+      sc.load(found, scales, row_scales, 0, sc.b0, blocks, count * NS);
+      if(!(ok = mbar_wait(empty + st, phase, g.status))) break;
+      if(tc::elect()) {
+         mbar_expect_tx(full + st, g.lags * (NS * g.row_bytes + (HEAD ? 0 : g.tap_bytes)));
+         if(!HEAD) load_taps(taps_map, at, 0, c0 / (128 / (int)sizeof(TT)), (int)j0, full + st);
+      }
+      __syncwarp();
+      for(int pair = lane * 4; pair < g.lags * NS; pair += 128)
+         gather4(codes_map, at + g.codes_at + pair * g.row_bytes, x, *reinterpret_cast<const int4*>(found + pair), full + st);
+      __syncwarp();
+      uint32_t seen = sc.store(entry, out, 0, sc.b0, blocks);
+      seen |= sc.rest(found, entry, scales, row_scales, out, blocks, count * NS);
+      seen = __reduce_or_sync(0xffffffffu, seen) & (NO_HALF | NO_ROW);
+      if constexpr(HEAD)
+         stage_taps(static_cast<const TT*>(a.taps) + j0 * a.taps_stride, a.taps_stride, c0, a.group, reinterpret_cast<float*>(at),
+                    g.tap_bytes / 4, blocks, count, lane);
+      if(lane == 0) flags[st] = seen | (uint32_t)count;
+      __syncwarp();
+      if(lane == 0) arrive(full + st);
+   }
+   if(!ok) {   // a wait gave up: time for the copies under way to land
+      const uint64_t t0 = globaltimer_ns();
+      while(globaltimer_ns() - t0 < 2000000ull) {}
+   }
+}
+
+// TT: of the taps; HEAD: shared by blocks of 32 channels; NS sequences a CTA
+template<bool MX8, class TT, bool HEAD, int NS>
+__global__ void __launch_bounds__(THREADS, 1) conv_pipe_kernel(const __grid_constant__ CUtensorMap codes_map,
+                                                               const __grid_constant__ CUtensorMap taps_map, Pages p, Args g)
+{
+   extern __shared__ uint8_t raw[];
+   uint8_t* ring = reinterpret_cast<uint8_t*>(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+   __shared__ uint64_t full[MAX_STAGES], empty[MAX_STAGES];
+   __shared__ uint32_t flags[MAX_STAGES], entry[256];   // lags of a stage, with NO_HALF and NO_ROW where one of its scales has it
+   __shared__ __align__(16) int rows[PRODUCERS][MAX_PAIRS];
+   const ConvStep& a = g.a;
+   const int warp = tc::uniform_warp(), lane = threadIdx.x & 31;
+   const int rank = a.split > 1 ? (int)tc::cluster_rank() : 0;
+   const int worker = blockIdx.x, workers = a.split * a.outer;
+   const int c0 = blockIdx.y * a.lanes * CH, b0 = blockIdx.z * NS;
+   const int units = min(a.lanes, a.channels / CH - (int)blockIdx.y * a.lanes), blocks = units / 2;
+
+   // the length of sequence lane % NS, and the longest of the NS, within the taps
+   const int mine = b0 + lane % NS < p.batch ? max(a.lengths[b0 + lane % NS], 0) : 0;
+   const int longest = min((int)__reduce_max_sync(0xffffffffu, (unsigned)mine), a.n_taps);
+   const int tiles = (int)(((long long)longest + g.lags - 1) / g.lags), n = tiles > worker ? (tiles - 1 - worker) / workers + 1 : 0;
+   if(threadIdx.x == 0) {
+      for(int s = 0; s < g.stages; ++s) {
+         mbar_init(full + s, 2);
+         mbar_init(empty + s, CONSUMERS);
+      }
+      fence_mbar_init();
+      prefetch_tmap(&codes_map);
+      if(!HEAD) prefetch_tmap(&taps_map);
+   }
+   if(threadIdx.x < 256) entry[threadIdx.x] = scale_entry(threadIdx.x);
+   __syncthreads();
+
+   float2 acc[NS][CH / 2];
+#pragma unroll
+   for(int s = 0; s < NS; ++s)
+#pragma unroll
+      for(int i = 0; i < CH / 2; ++i) acc[s][i] = make_float2(0.0f, 0.0f);
+   const int slots = a.slots, unit = threadIdx.x % a.lanes, slot = threadIdx.x / a.lanes;
+   const bool sums = warp < CONSUMERS && slot < slots && unit < units;
+
+   if(warp >= CONSUMERS) {
+      // Finding a stage's rows, issuing its copies and reading its scales take a warp as long as several stages
+      // take the sums, so several warps fill.  A slot of the ring is one warp's alone: a second one could wait
+      // for the slot's next phase while the first still waits for this one, and take this one's parity for it.
+      const int st = warp - CONSUMERS, x = (MX8 ? c0 : c0 / 2) / 4;
+      if(st < g.stages) {
+         if(g.quads) fill<TT, HEAD, NS, 4>(&codes_map, &taps_map, p, g, ring, full, empty, flags, entry, rows[st], st, n, worker, workers, longest, mine, b0, c0, x, blocks, lane);
+         else fill<TT, HEAD, NS, 1>(&codes_map, &taps_map, p, g, ring, full, empty, flags, entry, rows[st], st, n, worker, workers, longest, mine, b0, c0, x, blocks, lane);
+      }
+   } else {
+      Path w;
+      w.slot = slot;
+      w.slots = slots;
+      w.blocks = blocks;
+      w.row = g.row_bytes;
+      w.tap = slot * g.tap_bytes + (HEAD ? unit / 2 * 4 : unit * (CH * (int)sizeof(TT)));
+      w.tap_step = slots * g.tap_bytes;
+      w.codes = g.codes_at + slot * NS * g.row_bytes + unit * (MX8 ? CH : CH / 2);
+      w.codes_step = slots * NS * g.row_bytes;
+      w.scales = g.scales_at + (slot * NS * blocks + unit / 2) * 4;
+      w.scales_step = slots * NS * blocks;
+      int st = 0;
+      uint32_t phase = 0;
+      const uint8_t* at = ring;
+      for(int i = 0; i < n; ++i) {
+         if(!mbar_wait(full + st, phase, g.status)) break;
+         const uint32_t f = flags[st];
+         const int count = f & 0xffff;
+         if(sums) {
+            if(f <= 0xffff) sum_stage<MX8, TT, HEAD, NS, true>(at, w, count, acc);
+            else sum_stage<MX8, TT, HEAD, NS, false>(at, w, count, acc);
+         }
+         __syncwarp();
+         if(lane == 0) arrive(empty + st);
+         at += g.stage_bytes;
+         if(++st == g.stages) {
+            st = 0;
+            phase ^= 1;
+            at = ring;
+         }
+      }
+   }
+   __syncthreads();   // the ring is done with: every stage that was filled has been waited for
+   float* joined = reinterpret_cast<float*>(ring);
+   if(warp < CONSUMERS && slot < slots) park<NS>(joined, acc, slot, unit, slots, a.lanes);
+   join<NS>(joined, a, p, a.lanes * CH, slots, THREADS, rank, b0, c0);
+}
+
+struct Plan {
+   int ns, lanes, chunks, slots, split, outer, lags, stages;
+   int row_bytes, tap_bytes, codes_at, scales_at, stage_bytes;
+};
+constexpr int SMEM = 200 * 1024;
+
+// false: not this way.  tap_size: bytes of a tap, 0 where heads share them
+bool plan(long long lags, bool mx8, int channels, int batch, int tap_size, int sms, Plan* p)
+{
+   constexpr int grain = 4;   // units of a chunk: 128 bytes of taps, and of four rows of codes
+   const int units = channels / CH;
+   if(units % grain || units * (mx8 ? CH : CH / 2) < 256 || lags < 64) return false;
+   p->ns = batch > 2 ? 4 : batch;
+   const long long groups = mx::ceil_div(batch, p->ns);
+   // A cluster of eight joins short histories in the same launch; long ones
+   // are split over as many CTAs as the card takes at once, and joined by a
+   // second launch.
+   const double value = mx8 ? 33.0 / 32 : 17.0 / 32;
+   const bool small = (double)lags * channels * (batch * value + tap_size) < 64.0 * (1 << 20);
+   // scales that have to be read byte by byte are worth it for long histories only (5 x 5000 x 2112 MX4: 105 us, 65
+   // without the ring)
+   if(small && channels % 128) return false;
+   const auto lay = [&](int chunks) {
+      p->lanes = (int)mx::ceil_div(mx::ceil_div(units, chunks), grain) * grain;
+      p->chunks = (int)mx::ceil_div(units, p->lanes);
+      const int most = small ? MAX_SPLIT : (int)mx::ceil_div(lags, 256);
+      int w = (int)std::max<long long>(1, std::min<long long>(most, sms / (p->chunks * groups)));
+      if(small)
+         while(w & (w - 1)) w &= w - 1;   // clusters of 1, 2, 4 or 8
+      p->split = small ? w : 1;
+      p->outer = small ? 1 : w;
+      p->row_bytes = p->lanes * (mx8 ? CH : CH / 2);
+      p->tap_bytes = tap_size ? p->lanes * CH * tap_size : p->lanes / 2 * 4;
+      const int per_lag = p->tap_bytes + p->ns * (p->row_bytes + p->lanes / 2 * 4);
+      p->lags = 8;
+      // the scales of a stage are loaded in batches, one after the other where they are read byte by byte
+      const int rows = channels % 128 == 0 && p->lanes % 8 == 0 ? MAX_PAIRS : 64;
+      while(p->lags < 64 && p->lags * 2 * per_lag <= 44 * 1024 && p->lags * 2 * p->ns <= rows && lags >= (long long)p->lags * 4 * w)
+         p->lags *= 2;
+      p->slots = std::min(p->lags, CONSUMERS * 32 / p->lanes);
+      p->codes_at = (int)mx::ceil_div(p->lags * p->tap_bytes, 128) * 128;
+      p->scales_at = p->codes_at + p->lags * p->ns * p->row_bytes;
+      p->stage_bytes = (int)mx::ceil_div(p->lags * per_lag + 128, 1024) * 1024;
+      p->stages = std::min(MAX_STAGES, SMEM / p->stage_bytes);
+      return p->chunks * groups * w;   // CTAs
+   };
+   // chunks of 1024 channels, or of fewer where the card would not be full or the ring not four stages long
+   int chunks = (int)mx::ceil_div(units, 64);
+   while((lay(chunks) < sms * 3 / 4 || p->stages < 4) && units / (chunks * 2) >= 2 * grain) chunks *= 2;
+   lay(chunks);
+   return p->stages >= 3;
+}
+
+size_t smem_of(const Plan& p)
+{
+   const size_t ring = (size_t)p.stages * p.stage_bytes, sums = (size_t)p.ns * p.slots * p.lanes * CH * sizeof(float);
+   return std::max(ring, sums) + 1024;
+}
+
+template<bool MX8, class TT, bool HEAD, int NS>
+fufft_status launch(const fufft_cache* c, const Args& g, const CUtensorMap& cm, const CUtensorMap& tm, const Plan& p, cudaStream_t st)
+{
+   auto kern = conv_pipe_kernel<MX8, TT, HEAD, NS>;
+   static std::atomic<uint64_t> configured{0};
+   fufft_status s = allow_smem(kern, SMEM + 1024, configured);
+   if(s != FUFFT_OK) return s;
+   cudaLaunchConfig_t cfg = {};
+   cfg.gridDim = dim3((unsigned)(p.split * p.outer), (unsigned)p.chunks, (unsigned)mx::ceil_div(c->batch, NS));
+   cfg.blockDim = dim3(THREADS);
+   cfg.dynamicSmemBytes = smem_of(p);
+   cfg.stream = st;
+   cudaLaunchAttribute at[1];
+   at[0].id = cudaLaunchAttributeClusterDimension;
+   at[0].val.clusterDim.x = (unsigned)p.split;
+   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+   cfg.attrs = at;
+   cfg.numAttrs = 1;
+   if((s = check(cudaLaunchKernelEx(&cfg, kern, cm, tm, Pages(c), g))) != FUFFT_OK) return s;
+   count_launch();
+   return FUFFT_OK;
+}
+template<bool MX8, class TT, bool HEAD>
+fufft_status launch(const fufft_cache* c, const Args& g, const CUtensorMap& cm, const CUtensorMap& tm, const Plan& p, cudaStream_t st)
+{
+   return p.ns == 4 ? launch<MX8, TT, HEAD, 4>(c, g, cm, tm, p, st)
+                    : p.ns == 2 ? launch<MX8, TT, HEAD, 2>(c, g, cm, tm, p, st) : launch<MX8, TT, HEAD, 1>(c, g, cm, tm, p, st);
+}
+template<bool MX8, class TT>
+fufft_status launch(const fufft_cache* c, const Args& g, bool shared, const CUtensorMap& cm, const CUtensorMap& tm, const Plan& p,
+                    cudaStream_t st)
+{
+   return shared ? launch<MX8, TT, true>(c, g, cm, tm, p, st) : launch<MX8, TT, false>(c, g, cm, tm, p, st);
+}
+
+// taps as [lag][128 bytes][...]: boxes of a stage's lags and a chunk's channels, the 16-byte chunks of the
+// 128-byte rows permuted; lags beyond the last read as zeros
+fufft_status taps_tmap(CUtensorMap* tm, const ConvStep& a, int tap_size, const Plan& p)
+{
+   cuuint64_t dims[3] = {(cuuint64_t)(128 / tap_size), (cuuint64_t)(a.channels * tap_size / 128), (cuuint64_t)a.n_taps};
+   cuuint64_t strides[2] = {128, (cuuint64_t)a.taps_stride * tap_size};
+   cuuint32_t box[3] = {(cuuint32_t)(128 / tap_size), (cuuint32_t)(p.tap_bytes / 128), (cuuint32_t)p.lags};
+   return encode_tmap(tm, tap_size == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, a.taps, dims,
+                      strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// the cache's rows of codes, a box of one row's chunk
+fufft_status codes_tmap(CUtensorMap* tm, const fufft_cache* c, const Plan& p)
+{
+   const long long row = c->kind == FUFFT_CACHE_MX8 ? c->channels : c->channels / 2;
+   const cuuint64_t dims[2] = {(cuuint64_t)row / 4, (cuuint64_t)c->pages * c->page_size}, strides[1] = {(cuuint64_t)row};
+   const cuuint32_t box[2] = {(cuuint32_t)p.row_bytes / 4, 1};
+   return encode_tmap(tm, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, c->codes, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+}  // namespace pipe
 
 // How the work is laid out, from the sizes alone.
 struct Plan {
@@ -247,7 +748,7 @@ Plan plan(long long lags, int channels, int batch, int sms)
    const long long groups = mx::ceil_div(batch, p.nb);
    // clusters along the lags while a CTA keeps 32 of them
    p.split = 1;
-   while(p.split < 8 && lags >= 64ll * p.split) p.split *= 2;
+   while(p.split < MAX_SPLIT && lags >= 64ll * p.split) p.split *= 2;
    // channels in as few chunks as give four CTAs per SM, a chunk not below 256 channels
    p.chunks = (int)mx::ceil_div(units, THREADS);
    while(p.chunks * groups * p.split < 4ll * sms && mx::ceil_div(units, p.chunks * 2) >= 16) p.chunks *= 2;
@@ -279,11 +780,7 @@ fufft_status launch(const fufft_cache* c, const ConvStep& a, const Plan& p, cuda
    cfg.numAttrs = 1;
    if((s = check(cudaLaunchKernelEx(&cfg, kern, Pages(c), a))) != FUFFT_OK) return s;
    count_launch();
-   if(p.outer > 1) {
-      conv_join_kernel<<<(unsigned)mx::ceil_div((long long)c->batch * c->channels, 256), 256, 0, st>>>(a, c->batch);
-      count_launch();
-   }
-   return check(cudaGetLastError());
+   return FUFFT_OK;
 }
 template<bool MX8, class TT, Taps MODE>
 fufft_status launch(const fufft_cache* c, const ConvStep& a, const Plan& p, cudaStream_t st)
@@ -305,9 +802,17 @@ long long lags_of(const fufft_cache* c, int64_t n_taps)
    return held < n_taps ? held : n_taps;
 }
 
-size_t workspace(const Plan& p, const fufft_cache* c)
+// bytes of the partial results of `outer` clusters
+size_t partials(int outer, const fufft_cache* c)
 {
-   return p.outer == 1 ? 0 : (size_t)p.outer * c->batch * c->channels * sizeof(float);
+   return outer == 1 ? 0 : (size_t)outer * c->batch * c->channels * sizeof(float);
+}
+
+fufft_status join_clusters(const ConvStep& a, int batch, cudaStream_t st)
+{
+   conv_join_kernel<<<(unsigned)mx::ceil_div((long long)batch * a.channels, 256), 256, 0, st>>>(a, batch);
+   count_launch();
+   return check(cudaGetLastError());
 }
 
 }  // namespace cache
@@ -320,8 +825,13 @@ size_t fufft_cache_conv_workspace(const fufft_cache* c, int64_t n_taps)
    if(cache::check_cache(c) != FUFFT_OK || n_taps < 0 || n_taps > cache::MAX_TOKENS || c->batch == 0) return 0;
    int dev = 0;
    if(cudaGetDevice(&dev) != cudaSuccess) return 0;
-   const cache::Plan p = cache::plan(cache::lags_of(c, n_taps), c->channels, c->batch, sm_count(dev));
-   return cache::workspace(p, c);
+   const long long lags = cache::lags_of(c, n_taps);
+   const int sms = sm_count(dev);
+   int outer = cache::plan(lags, c->channels, c->batch, sms).outer;
+   cache::pipe::Plan p;   // whichever way the taps will lie
+   for(int tap_size : {0, 2, 4})
+      if(cache::pipe::plan(lags, c->kind == FUFFT_CACHE_MX8, c->channels, c->batch, tap_size, sms, &p)) outer = std::max(outer, p.outer);
+   return cache::partials(outer, c);
 }
 
 fufft_status fufft_cache_conv(const fufft_cache* c, const int32_t* lengths, const void* taps, fufft_dtype taps_dtype,
@@ -343,9 +853,6 @@ fufft_status fufft_cache_conv(const fufft_cache* c, const int32_t* lengths, cons
       return FUFFT_ERR_MISALIGNED;
    int dev = 0;
    if((s = check(cudaGetDevice(&dev))) != FUFFT_OK) return s;
-   const cache::Plan p = cache::plan(cache::lags_of(c, n_taps), c->channels, c->batch, sm_count(dev));
-   const size_t need = cache::workspace(p, c);
-   if(workspace_bytes < need || (need && !workspace)) return FUFFT_ERR_INVALID_ARG;
    cache::ConvStep a{};
    a.lengths = lengths;
    a.taps = taps;
@@ -358,17 +865,47 @@ fufft_status fufft_cache_conv(const fufft_cache* c, const int32_t* lengths, cons
    a.out = out;
    a.out_stride = out_stride;
    a.dtype = dtype;
-   a.vec_taps = aligned(taps, 16) && taps_stride * (taps_dtype == FUFFT_F32 ? 4 : 2) % 16 == 0;
+   const int tap_size = taps_dtype == FUFFT_F32 ? 4 : 2;
+   a.vec_taps = aligned(taps, 16) && taps_stride * tap_size % 16 == 0;
+   const bool mx8 = c->kind == FUFFT_CACHE_MX8;
+   const long long lags = cache::lags_of(c, n_taps);
+   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+
+   // long rows, taps that a tensor copy takes or that whole blocks share: the ring
+   cache::pipe::Plan pp;
+   const bool shared = a.group % mx::BLOCK == 0;
+   if((shared || (a.group == 1 && a.vec_taps)) &&
+      c->pages > 0 && cache::pipe::plan(lags, mx8, c->channels, c->batch, shared ? 0 : tap_size, sm_count(dev), &pp)) {
+      const size_t need = cache::partials(pp.outer, c);
+      if(workspace_bytes < need || (need && !workspace)) return FUFFT_ERR_INVALID_ARG;
+      DeviceCtx ctx;
+      if((s = device_ctx(&ctx)) != FUFFT_OK) return s;
+      a.partial = need ? static_cast<float*>(workspace) : nullptr;
+      a.lanes = pp.lanes;
+      a.slots = pp.slots;
+      a.split = pp.split;
+      a.outer = pp.outer;
+      CUtensorMap tm{}, cm;
+      if((s = cache::pipe::codes_tmap(&cm, c, pp)) != FUFFT_OK) return s;
+      if(!shared && (s = cache::pipe::taps_tmap(&tm, a, tap_size, pp)) != FUFFT_OK) return s;
+      const cache::pipe::Args g{a, ctx.status, pp.lags, pp.stages, pp.stage_bytes, pp.codes_at, pp.scales_at, pp.row_bytes, pp.tap_bytes,
+                                c->channels % 128 == 0 && pp.lanes % 8 == 0};
+      if(mx8) s = tap_size == 4 ? cache::pipe::launch<true, float>(c, g, shared, cm, tm, pp, st) : cache::pipe::launch<true, __nv_bfloat16>(c, g, shared, cm, tm, pp, st);
+      else s = tap_size == 4 ? cache::pipe::launch<false, float>(c, g, shared, cm, tm, pp, st) : cache::pipe::launch<false, __nv_bfloat16>(c, g, shared, cm, tm, pp, st);
+      return s != FUFFT_OK || pp.outer == 1 ? s : cache::join_clusters(a, c->batch, st);
+   }
+   const cache::Plan p = cache::plan(lags, c->channels, c->batch, sm_count(dev));
+   const size_t need = cache::partials(p.outer, c);
+   if(workspace_bytes < need || (need && !workspace)) return FUFFT_ERR_INVALID_ARG;
    a.partial = need ? static_cast<float*>(workspace) : nullptr;
    a.lanes = p.lanes;
    a.slots = p.slots;
    a.split = p.split;
    a.outer = p.outer;
    a.tile = p.tile;
-   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-   if(c->kind == FUFFT_CACHE_MX8)
-      return taps_dtype == FUFFT_F32 ? cache::launch<true, float>(c, a, p, st) : cache::launch<true, __nv_bfloat16>(c, a, p, st);
-   return taps_dtype == FUFFT_F32 ? cache::launch<false, float>(c, a, p, st) : cache::launch<false, __nv_bfloat16>(c, a, p, st);
+   if(mx8) s = tap_size == 4 ? cache::launch<true, float>(c, a, p, st) : cache::launch<true, __nv_bfloat16>(c, a, p, st);
+   else s = tap_size == 4 ? cache::launch<false, float>(c, a, p, st) : cache::launch<false, __nv_bfloat16>(c, a, p, st);
+   return s != FUFFT_OK || p.outer == 1 ? s : cache::join_clusters(a, c->batch, st);
 }
 
 }  // extern "C"

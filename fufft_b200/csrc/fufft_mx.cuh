@@ -36,6 +36,9 @@ template<class K> fufft_status allow_smem(K kern, int bytes, std::atomic<uint64_
    if(s == FUFFT_OK) done.fetch_or(bit, std::memory_order_acq_rel);
    return s;
 }
+// tiled tensor map with unit element strides and zero fill; FUFFT_ERR_UNSUPPORTED where the driver refuses it
+fufft_status encode_tmap(CUtensorMap* tm, CUtensorMapDataType type, int rank, const void* base, const cuuint64_t* dims,
+                         const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle);
 }  // namespace host
 namespace mx {
 

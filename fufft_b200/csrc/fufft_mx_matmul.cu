@@ -2,10 +2,7 @@
 // out[m][n] = sum_k a[m][k] b[n][k] + bias[n], on the tensor cores
 // (tcgen05 kind::mxf4: E2M1 products under E8M0 scales, fp32 sums in tensor
 // memory).
-#include <cudaTypedefs.h>
-
 #include <algorithm>
-#include <mutex>
 
 #include "fufft_internal.cuh"
 #include "fufft_mx.cuh"
@@ -452,48 +449,20 @@ __global__ void __launch_bounds__(P::THREADS, 1) matmul_pair_kernel(const __grid
    if(warp == 1) tc::tmem_free_pair<P::TMEM>(tmem);
 }
 
-PFN_cuTensorMapEncodeTiled_v12000 tmap_encoder()
-{
-   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-   static std::once_flag once;
-   std::call_once(once, [] {
-      void* p = nullptr;
-      cudaDriverEntryPointQueryResult q;
-      if(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-         q == cudaDriverEntryPointSuccess)
-         fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-   });
-   return fn;
-}
-
 // 4-bit codes as tiles of box_rows x 128 bytes, 128-byte swizzle; rows beyond the last read as zeros
 fufft_status codes_tmap(CUtensorMap* tm, const uint8_t* codes, long long rows, long long pitch, int box_rows)
 {
-   const auto fn = tmap_encoder();
-   if(!fn) return FUFFT_ERR_UNSUPPORTED;
-   cuuint64_t dims[2] = {(cuuint64_t)pitch, (cuuint64_t)rows};
-   cuuint64_t strides[1] = {(cuuint64_t)pitch};
-   cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
-   cuuint32_t estr[2] = {1, 1};
-   const CUresult r = fn(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(codes), dims, strides, box, estr,
-                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-   return r == CUDA_SUCCESS ? FUFFT_OK : FUFFT_ERR_UNSUPPORTED;
+   const cuuint64_t dims[2] = {(cuuint64_t)pitch, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)pitch};
+   const cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+   return encode_tmap(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, codes, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 // the scale tiles of 128 rows x 256 columns, 1024 bytes each as 256 words; tiles beyond the last row read as zeros
 fufft_status scales_tmap(CUtensorMap* tm, const uint8_t* scales, long long rows, int chunks)
 {
-   const auto fn = tmap_encoder();
-   if(!fn) return FUFFT_ERR_UNSUPPORTED;
-   cuuint64_t dims[2] = {(cuuint64_t)chunks * 256, (cuuint64_t)ceil_div(rows, TILE_ROWS)};
-   cuuint64_t strides[1] = {(cuuint64_t)chunks * 1024};
-   cuuint32_t box[2] = {256, 1};
-   cuuint32_t estr[2] = {1, 1};
-   const CUresult r = fn(tm, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<uint8_t*>(scales), dims, strides, box, estr,
-                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-   return r == CUDA_SUCCESS ? FUFFT_OK : FUFFT_ERR_UNSUPPORTED;
+   const cuuint64_t dims[2] = {(cuuint64_t)chunks * 256, (cuuint64_t)ceil_div(rows, TILE_ROWS)}, strides[1] = {(cuuint64_t)chunks * 1024};
+   const cuuint32_t box[2] = {256, 1};
+   return encode_tmap(tm, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, scales, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
 struct Operands {

@@ -1,5 +1,9 @@
 // fufft_mx_quant.cu -- 4-bit microscaled matrices: quantisation along the
 // rows, along the columns, or both from one read, and the way back.
+#include <cudaTypedefs.h>
+
+#include <mutex>
+
 #include "fufft_internal.cuh"
 #include "fufft_mx.cuh"
 #include "fufft_tc.cuh"
@@ -8,6 +12,26 @@ using namespace fufft;
 using namespace fufft::host;
 
 namespace fufft {
+namespace host {
+fufft_status encode_tmap(CUtensorMap* tm, CUtensorMapDataType type, int rank, const void* base, const cuuint64_t* dims,
+                         const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle)
+{
+   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+   static std::once_flag once;
+   std::call_once(once, [] {
+      void* p = nullptr;
+      cudaDriverEntryPointQueryResult q;
+      if(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+         q == cudaDriverEntryPointSuccess)
+         fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+   });
+   if(!fn) return FUFFT_ERR_UNSUPPORTED;
+   const cuuint32_t ones[5] = {1, 1, 1, 1, 1};
+   const CUresult r = fn(tm, type, (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+   return r == CUDA_SUCCESS ? FUFFT_OK : FUFFT_ERR_UNSUPPORTED;
+}
+}  // namespace host
 namespace mx {
 
 // Alignment of the rows of a matrix: whole 32-byte transfers, or any.

@@ -144,7 +144,9 @@ def test_append_strided(ops):
 STEPS = [(1, [1], 32, 16, 1, 32), (1, [700], 64, 16, 700, 64), (3, [0, 5, 33], 96, 48, 20, 3), (2, [64, 65], 1056, 64, 300, 1056),
          (5, [100, 0, 257, 31, 1], 288, 100, 256, 9), (9, [300, 299, 1, 2, 0, 128, 64, 200, 17], 128, 7, 129, 128),
          (1, [5000], 256, 64, 4999, 1), (2, [1500, 800], 2080, 64, 1024, 65), (17, [90 - 5 * i for i in range(17)], 32, 16, 64, 16),
-         (2, [400, 401], 96, 16, 350, 32), (3, [70, 90, 200], 96, 16, 150, 8), (4, [0, 0, 0, 0], 64, 16, 10, 64)]
+         (2, [400, 401], 96, 16, 350, 32), (3, [70, 90, 200], 96, 16, 150, 8), (4, [0, 0, 0, 0], 64, 16, 10, 64),
+         (6, [1000, 0, 333, 999, 64, 1], 1024, 64, 900, 1024), (3, [300, 299, 2], 2048, 16, 300, 2048), (1, [513], 1088, 100, 700, 1088),
+         (2, [0, 0], 512, 64, 200, 512), (4, [129, 128, 127, 0], 3200, 64, 128, 100)]
 
 
 def _step(m, taps, gate, dtype):
@@ -176,6 +178,52 @@ def test_conv(ops, step, dtype, kind):
         assert got.dtype == dtype
         err = (got.cpu().double() - want).abs()
         assert bool((err <= tol).all()), float((err - tol).max())
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+def test_conv_missing_pages_in_long_rows(ops, kind):
+    """pages that are not there, and codes beside them that are NaN (mx8) or anything (mx4), add nothing"""
+    m = Model(ops, 4, 400, 1024, 16, kind, seed=21)
+    m.append([400, 399, 17, 200], torch.float32)
+    taps = torch.randn(350, 1024, generator=m.g)
+    for b, k in ((0, 24), (0, 3), (1, 0), (1, 10), (3, 12)):      # page k of sequence b
+        m.cache.codes[m.cache.page_table[b, k].long()] = 0x7F
+        m.cache.page_table[b, k] = -1 if k % 2 else m.cache.codes.shape[0]
+        m.rows[b][16 * k:16 * k + 16] = 0.0
+    want, tol = _step(m, taps, None, torch.float32)
+    got = ops.cache_conv(m.cache, m.lengths.cuda(), taps.cuda(), dtype=torch.float32)
+    assert bool(((got.cpu().double() - want).abs() <= tol).all())
+    heads = torch.randn(350, 32, generator=m.g)
+    want, tol = _step(m, heads, None, torch.float32)
+    got = ops.cache_conv(m.cache, m.lengths.cuda(), heads.cuda(), dtype=torch.float32)
+    assert bool(((got.cpu().double() - want).abs() <= tol).all())
+
+
+@gpu
+@pytest.mark.parametrize("heads", [2048, 64, 2048 // 16])
+@pytest.mark.parametrize("kind", KINDS)
+def test_conv_long(ops, kind, heads):
+    """histories that several launches' worth of CTAs share; the reference from the values read back, in 64 bits"""
+    g = torch.Generator(device="cuda").manual_seed(31)
+    batch, n, channels, page = 5, 9000, 2048, 64
+    per = -(-n // page)
+    table = torch.randperm(batch * per, device="cuda", generator=g).view(batch, per).int()
+    cache = ops.seq_cache(batch * per, page, channels, table, kind)
+    lengths = torch.tensor([9000, 8999, 0, 4097, 100], dtype=torch.int32)
+    x = torch.randn(int(lengths.sum()), channels, device="cuda", generator=g)
+    cu, zero = _cu(lengths.tolist()).cuda(), torch.zeros(batch, dtype=torch.int32, device="cuda")
+    ops.cache_append(cache, x, cu, zero)
+    stored = ops.cache_read(cache, cu, zero, x.shape[0], torch.float32).split(lengths.tolist())
+    for taps_dtype in (torch.float32, torch.bfloat16):
+        taps = torch.randn(8500, heads, device="cuda", generator=g).to(taps_dtype)
+        got = ops.cache_conv(cache, lengths.cuda(), taps, dtype=torch.float32).double()
+        for b, v in enumerate(stored):
+            k = min(len(v), 8500)
+            t = v.flip(0)[:k].double() * taps[:k].double().repeat_interleave(channels // heads, 1)
+            tol = ref.sum_tolerance(t.sum(0), t.abs().sum(0), k, torch.float32)
+            assert bool(((got[b] - t.sum(0)).abs() <= tol).all())
+        assert torch.equal(ops.cache_conv(cache, lengths.cuda(), taps, dtype=torch.float32).double(), got)
 
 
 @gpu
