@@ -743,20 +743,26 @@ Plan plan(long long lags, int channels, int batch, int sms)
 {
    Plan p;
    lags = lags > 0 ? lags : 1;
-   p.nb = batch >= 3 ? 4 : batch;
    const int units = channels / CH;
-   const long long groups = mx::ceil_div(batch, p.nb);
    // clusters along the lags while a CTA keeps 32 of them
    p.split = 1;
    while(p.split < MAX_SPLIT && lags >= 64ll * p.split) p.split *= 2;
-   // channels in as few chunks as give four CTAs per SM, a chunk not below 256 channels
-   p.chunks = (int)mx::ceil_div(units, THREADS);
-   while(p.chunks * groups * p.split < 4ll * sms && mx::ceil_div(units, p.chunks * 2) >= 16) p.chunks *= 2;
-   p.lanes = (int)mx::ceil_div(units, p.chunks);
-   p.slots = THREADS / p.lanes;
-   p.outer = 1;
-   while(p.chunks * groups * p.split * p.outer < 2ll * sms && lags >= 2048ll * p.split * p.outer) p.outer *= 2;
-   p.tile = (int)std::min<long long>(TILE, mx::ceil_div(lags, (long long)p.split * p.outer));
+   // Channels in as few chunks as give four CTAs per SM, a chunk not below 256 channels; fewer sequences that share
+   // their taps where that leaves SMs without a pair of CTAs.
+   for(p.nb = batch > 2 ? 4 : batch;; p.nb /= 2) {
+      const long long groups = mx::ceil_div(batch, p.nb);
+      p.chunks = (int)mx::ceil_div(units, THREADS);
+      while(p.chunks * groups * p.split < 4ll * sms && mx::ceil_div(units, p.chunks * 2) >= 16) p.chunks *= 2;
+      p.lanes = (int)mx::ceil_div(units, p.chunks);
+      p.chunks = (int)mx::ceil_div(units, p.lanes);
+      p.slots = THREADS / p.lanes;
+      p.outer = 1;
+      while(p.chunks * groups * p.split * p.outer < 2ll * sms && lags >= 2048ll * p.split * p.outer) p.outer *= 2;
+      if(p.nb == 1 || p.chunks * groups * p.split * p.outer >= 2ll * sms) break;
+   }
+   // the same number of tiles for every CTA
+   const long long workers = (long long)p.split * p.outer, tiles = mx::ceil_div(lags, workers * TILE);
+   p.tile = (int)mx::ceil_div(lags, workers * tiles);
    return p;
 }
 
