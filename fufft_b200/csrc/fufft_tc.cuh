@@ -126,6 +126,18 @@ __device__ __forceinline__ bool elect()
    return p != 0;
 }
 
+// ---- tiles on their way out ---------------------------------------------------
+// 2-D tile from shared memory; what lies outside the tensor is left out.  x, y not negative, x a multiple of 16 bytes
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* tm, int x, int y, const void* src)
+{
+   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];"
+                :: "l"(tm), "r"(smem_u32(src)), "r"(x), "r"(y) : "memory");
+   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// this thread's stores have been read out of shared memory / have been done
+__device__ __forceinline__ void tma_stores_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void tma_stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
 // ---- programmatic dependent launch -----------------------------------------
 // the next kernel of the stream, if it was launched so, may be scheduled from here on
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;"); }
