@@ -284,10 +284,6 @@ struct Args {
    bool quads;                                           // four blocks' scales at once
 };
 
-__device__ __forceinline__ void arrive(uint64_t* bar)
-{
-   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(smem_u32(bar)) : "memory");
-}
 __device__ __forceinline__ void load_taps(const CUtensorMap* tm, void* dst, int x, int y, int z, uint64_t* bar)
 {
    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
@@ -523,7 +519,7 @@ __device__ __forceinline__ void fill(const CUtensorMap* codes_map, const CUtenso
                     g.tap_bytes / 4, blocks, count, lane);
       if(lane == 0) flags[st] = seen | (uint32_t)count;
       __syncwarp();
-      if(lane == 0) arrive(full + st);
+      if(lane == 0) tc::arrive_own(full + st);
    }
    if(!ok) {   // a wait gave up: time for the copies under way to land
       const uint64_t t0 = globaltimer_ns();
@@ -605,7 +601,7 @@ __global__ void __launch_bounds__(THREADS, 1) conv_pipe_kernel(const __grid_cons
             else sum_stage<MX8, TT, HEAD, NS, false>(at, w, count, acc);
          }
          __syncwarp();
-         if(lane == 0) arrive(empty + st);
+         if(lane == 0) tc::arrive_own(empty + st);
          at += g.stage_bytes;
          if(++st == g.stages) {
             st = 0;

@@ -3,6 +3,7 @@
 // (tcgen05 kind::mxf4: E2M1 products under E8M0 scales, fp32 sums in tensor
 // memory).
 #include <algorithm>
+#include <type_traits>
 
 #include "fufft_internal.cuh"
 #include "fufft_mx.cuh"
@@ -30,7 +31,21 @@ struct MatmulArgs {
 // still streams b at full width, and CTAs of a cluster take parts of the
 // summed axis and join their sums through distributed shared memory, in rank
 // order.  Bound by reading b's codes and scales once.
+//
+// Rows that are not quantised yet (Raw<X>, sixteen at most) are quantised on
+// the way: two warps that have nothing else to do put each stage's 256 columns
+// into the layout that the copies would have left, in every CTA that needs
+// them; a launch and its wait less (one token 4096 x 4096: 7.5 us with the
+// quantiser's launch, 5.5 so).
 // ---------------------------------------------------------------------------
+struct Packed {};              // a comes in codes and scales
+template<class X> struct Raw {}; // a comes as rows of X
+struct RawArgs {
+   const void* x;
+   long long stride, cols;
+   bool on_32;
+};
+
 constexpr int MAX_SPLIT = 8;         // CTAs of a portable cluster
 template<int BN> struct Split {
    static constexpr int SF_Q = (BN + 127) / 128;                     // scale tiles of the columns
@@ -47,11 +62,41 @@ template<int BN> struct Split {
    static_assert(STAGE % 1024 == 0, "the 128-byte swizzle repeats every 1024 bytes");
 };
 
-template<class T, int BN>
+// A stage's columns of the unquantised rows, by 64 threads: a thread takes half
+// blocks of 16 values, two neighbouring lanes a block.
+template<class X>
+__device__ __forceinline__ void quantize_stage(const RawArgs& r, int rows, long long col0, uint8_t* codes, uint8_t* scales, int thread)
+{
+   Half<X> h[4];
+#pragma unroll
+   for(int u = 0; u < 4; ++u) {
+      const int row = u * 4 + (thread >> 4);
+      const long long col = col0 + (thread & 15) * HALF;
+      const int count = row < rows ? (int)max(0ll, min((long long)HALF, r.cols - col)) : 0;
+      const X* at = static_cast<const X*>(r.x) + row * r.stride + col;
+      if(r.on_32 && count == HALF) h[u].load(at);
+      else h[u].load_some(at, count);
+   }
+#pragma unroll
+   for(int u = 0; u < 4; ++u) {
+      const int row = u * 4 + (thread >> 4), half = thread & 15;
+      uint32_t q[2];
+      const uint32_t s = encode_pair<false>(h[u], q);
+      // 128-byte rows whose 16-byte chunks are permuted by the row, as the copies' swizzle leaves them
+      *reinterpret_cast<uint2*>(codes + row * 128 + ((half >> 1 ^ (row & 7)) << 4) + (half & 1) * 8) = make_uint2(q[0], q[1]);
+      if((half & 1) == 0) scales[(half >> 3) * TILE_BYTES + tile_word(row) + (half >> 1 & 3)] = (uint8_t)s;
+   }
+}
+template<class A> struct RowType { using type = float; };
+template<class X> struct RowType<Raw<X>> { using type = X; };
+
+template<class T, int BN, class A>
 __global__ void __launch_bounds__(128) matmul_split_kernel(const __grid_constant__ CUtensorMap tp,
-                                                           const __grid_constant__ CUtensorMap tq, MatmulArgs g)
+                                                           const __grid_constant__ CUtensorMap tq, MatmulArgs g, RawArgs x)
 {
    using C = Split<BN>;
+   constexpr bool PACKED = std::is_same_v<A, Packed>;
+   static_assert(PACKED || BN == 16, "sixteen rows at most are quantised here");
    extern __shared__ uint8_t raw[];
    uint8_t* body = reinterpret_cast<uint8_t*>(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
    uint64_t* full = reinterpret_cast<uint64_t*>(body + C::BODY);
@@ -69,7 +114,7 @@ __global__ void __launch_bounds__(128) matmul_split_kernel(const __grid_constant
 
    if(threadIdx.x == 0) {
       for(int s = 0; s < C::STAGES; ++s) {
-         mbar_init(full + s, 1);
+         mbar_init(full + s, PACKED ? 1 : 3);
          mbar_init(empty + s, 1);
       }
       mbar_init(done, 1);
@@ -91,7 +136,7 @@ __global__ void __launch_bounds__(128) matmul_split_kernel(const __grid_constant
       const uint8_t* p_scale = g.p_scale + ((long long)(p0 / TILE_ROWS) * g.chunks + k0) * C::SF_BYTES;
       const uint8_t* q_scale = g.q_scale + (q0 / TILE_ROWS * g.chunks + k0) * C::SF_BYTES;
       auto load_p = [&](int i, int s) {
-         mbar_expect_tx(full + s, C::STAGE);
+         mbar_expect_tx(full + s, PACKED ? C::STAGE : C::P_BYTES + C::SF_BYTES);
          tma_load_2d(body + s * C::STAGE, &tp, (k0 + i) * 128, p0, full + s);
          bulk_g2s(body + s * C::STAGE + C::P_BYTES + C::Q_BYTES, p_scale + (long long)i * C::SF_BYTES, C::SF_BYTES, full + s);
       };
@@ -107,9 +152,11 @@ __global__ void __launch_bounds__(128) matmul_split_kernel(const __grid_constant
       const int ahead = min(n, C::STAGES);
       if(tc::elect())
          for(int i = 0; i < ahead; ++i) load_p(i, i);
-      tc::wait_for_previous();
-      if(tc::elect())
-         for(int i = 0; i < ahead; ++i) load_q(i, i);
+      if constexpr(PACKED) {
+         tc::wait_for_previous();
+         if(tc::elect())
+            for(int i = 0; i < ahead; ++i) load_q(i, i);
+      }
       __syncwarp();
       int issued = ahead, s = 0;
       uint32_t phase = 0;
@@ -121,7 +168,7 @@ __global__ void __launch_bounds__(128) matmul_split_kernel(const __grid_constant
          }
          if(tc::elect()) {
             load_p(i, s);
-            load_q(i, s);
+            if(PACKED) load_q(i, s);
          }
          __syncwarp();
          issued = i + 1;
@@ -164,6 +211,22 @@ __global__ void __launch_bounds__(128) matmul_split_kernel(const __grid_constant
          }
       }
       if(tc::elect()) tc::commit(done);
+   } else if(!PACKED && warp >= 2) {
+      int s = 0;
+      uint32_t phase = 1;
+      for(int i = 0; i < n; ++i) {
+         if(!mbar_wait(empty + s, phase, g.status)) break;
+         uint8_t* at = body + s * C::STAGE + C::P_BYTES;
+         quantize_stage<typename RowType<A>::type>(x, (int)g.q_rows, (long long)(k0 + i) * K_PAD, at, at + C::Q_BYTES + C::SF_BYTES,
+                                                   threadIdx.x - 64);
+         fence_proxy_async_smem();
+         __syncwarp();
+         if(lane == 0) tc::arrive_own(full + s);
+         if(++s == C::STAGES) {
+            s = 0;
+            phase ^= 1;
+         }
+      }
    }
    __syncwarp();
    bool ok = n == 0 || mbar_wait(done, 0, g.status);
@@ -478,8 +541,8 @@ struct Operands {
    bool follows;             // the kernel before on the stream wrote a (and neither b nor anything else that is read)
 };
 
-template<class T, int BN>
-fufft_status launch_split(const Operands& o, int split, const DeviceCtx& ctx, cudaStream_t st)
+template<class T, int BN, class A = Packed>
+fufft_status launch_split(const Operands& o, int split, const DeviceCtx& ctx, cudaStream_t st, const RawArgs& x = {})
 {
    using C = Split<BN>;
    const long long pitch = mx4_pitch(o.k);
@@ -487,9 +550,9 @@ fufft_status launch_split(const Operands& o, int split, const DeviceCtx& ctx, cu
    fufft_status s;
    if(o.k) {
       if((s = codes_tmap(&tp, o.b, o.n, pitch, 128)) != FUFFT_OK) return s;
-      if((s = codes_tmap(&tq, o.a, o.m, pitch, BN)) != FUFFT_OK) return s;
+      if(std::is_same_v<A, Packed> && (s = codes_tmap(&tq, o.a, o.m, pitch, BN)) != FUFFT_OK) return s;
    }
-   auto kern = matmul_split_kernel<T, BN>;
+   auto kern = matmul_split_kernel<T, BN, A>;
    static std::atomic<uint64_t> configured{0};
    if((s = allow_smem(kern, C::SMEM, configured)) != FUFFT_OK) return s;
    MatmulArgs g{o.b_scale, o.a_scale, o.bias, o.out, ctx.status, o.n, o.m, o.out_stride, (int)(pitch / 128),
@@ -507,7 +570,7 @@ fufft_status launch_split(const Operands& o, int split, const DeviceCtx& ctx, cu
    at[1].val.programmaticStreamSerializationAllowed = 1;
    cfg.attrs = at;
    cfg.numAttrs = o.follows ? 2 : 1;
-   if((s = check(cudaLaunchKernelEx(&cfg, kern, tp, tq, g))) != FUFFT_OK) return s;
+   if((s = check(cudaLaunchKernelEx(&cfg, kern, tp, tq, g, x))) != FUFFT_OK) return s;
    count_launch();
    return check(cudaGetLastError());
 }
@@ -580,10 +643,12 @@ template<class T> fufft_status matmul(const Operands& o, cudaStream_t st)
    if(o.m <= 32) return launch_split<T, 32>(o, split_for(tiles_p, chunks, sms), ctx, st);
    if(o.m <= 64) return launch_split<T, 64>(o, split_for(tiles_p, chunks, sms), ctx, st);
    // Pairs, unless their tiles leave most of the card idle and a long summed
-   // axis pays for joining its parts (us, split / pair: 512 x 512 x 8192 9.7 /
-   // 13.1, 128 x 1024 x 1024 9.0 / 7.2, 333 x 1537 x 1111 9.4 / 9.1).
+   // axis pays for joining its parts, or where a small result's rows start
+   // anywhere (us, split / pair: 512 x 512 x 8192 9.7 / 13.1, 128 x 1024 x 1024
+   // 9.0 / 7.2, 333 x 1537 x 1111 9.4 / 12.0, 333 x 1536 x 1111 9.4 / 6.5).
+   const bool aligned_rows = aligned(o.out, 16) && o.out_stride * (long long)sizeof(T) % 16 == 0;
    const long long pairs = sms / 2, narrow = ceil_div(o.m, 256) * ceil_div(o.n, 192), wide = ceil_div(o.m, 256) * ceil_div(o.n, 256);
-   if(narrow * MAX_SPLIT <= pairs && chunks >= 8)
+   if((narrow * MAX_SPLIT <= pairs && chunks >= 8) || (narrow * 2 <= pairs && !aligned_rows))
       return launch_split<T, 128>(o, split_for(tiles_p * ceil_div(o.m, 128), chunks, sms), ctx, st);
    if(chunks == 0) return launch_split<T, 128>(o, 1, ctx, st);
    // 256 columns in one accumulator or 192 in two of them, whichever covers the
@@ -591,6 +656,21 @@ template<class T> fufft_status matmul(const Operands& o, cudaStream_t st)
    // 30.9 / 28.5, 512 x 4096 x 4096 11.8 / 10.1)
    return ceil_div(wide, pairs) * 256 < ceil_div(narrow, pairs) * 192 ? launch_pair<T, Pair<256, 1>>(o, ctx, st)
                                                                      : launch_pair<T, Pair<192, 2>>(o, ctx, st);
+}
+
+// rows of x quantised on the way
+template<class T>
+fufft_status matmul_raw(const Operands& o, fufft_dtype x_dtype, const RawArgs& x, cudaStream_t st)
+{
+   DeviceCtx ctx;
+   fufft_status s = device_ctx(&ctx);
+   if(s != FUFFT_OK) return s;
+   const int split = split_for(ceil_div(o.n, 128), (int)(mx4_pitch(o.k) / 128), sm_count(ctx.device));
+   switch(x_dtype) {
+   case FUFFT_F32: return launch_split<T, 16, Raw<float>>(o, split, ctx, st, x);
+   case FUFFT_F16: return launch_split<T, 16, Raw<__half>>(o, split, ctx, st, x);
+   default: return launch_split<T, 16, Raw<__nv_bfloat16>>(o, split, ctx, st, x);
+   }
 }
 
 fufft_status matmul(const Operands& o, fufft_dtype dtype, fufft_stream_t stream)
@@ -641,10 +721,24 @@ fufft_status fufft_mx4_linear(const void* x, fufft_dtype x_dtype, int64_t m, int
                               fufft_stream_t stream)
 {
    // everything is checked before the first launch: a refused call leaves x_codes alone
-   fufft_status s = check_matmul(x_codes, x_scales, w_codes, w_scales, bias, out, dtype, m, n, k, out_stride);
+   const bool direct = m <= FUFFT_MX4_DIRECT_ROWS;
+   fufft_status s = check_matmul(direct ? w_codes : x_codes, direct ? w_scales : x_scales, w_codes, w_scales, bias, out, dtype, m, n, k, out_stride);
    if(s != FUFFT_OK || m == 0 || n == 0) return s;
-   if((s = fufft_mx4_quantize(x, x_dtype, m, k, x_stride, x_codes, x_scales, nullptr, nullptr, stream)) != FUFFT_OK) return s;
-   return mx::matmul({x_codes, x_scales, w_codes, w_scales, bias, out, m, n, k, out_stride, k > 0}, dtype, stream);
+   if(!direct || k == 0) {
+      if((s = fufft_mx4_quantize(x, x_dtype, m, k, x_stride, x_codes, x_scales, nullptr, nullptr, stream)) != FUFFT_OK) return s;
+      return mx::matmul({x_codes, x_scales, w_codes, w_scales, bias, out, m, n, k, out_stride, k > 0}, dtype, stream);
+   }
+   if(x_dtype < FUFFT_F32 || x_dtype > FUFFT_BF16 || !x || (m > 1 && x_stride < k)) return FUFFT_ERR_INVALID_ARG;
+   const long long size = x_dtype == FUFFT_F32 ? 4 : 2;
+   if(!aligned(x, (unsigned)size)) return FUFFT_ERR_MISALIGNED;
+   const mx::Operands o{nullptr, nullptr, w_codes, w_scales, bias, out, m, n, k, out_stride, false};
+   const mx::RawArgs rows{x, x_stride, k, aligned(x, 32) && (m == 1 || x_stride * size % 32 == 0)};
+   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+   switch(dtype) {
+   case FUFFT_F32: return mx::matmul_raw<float>(o, x_dtype, rows, st);
+   case FUFFT_F16: return mx::matmul_raw<__half>(o, x_dtype, rows, st);
+   default: return mx::matmul_raw<__nv_bfloat16>(o, x_dtype, rows, st);
+   }
 }
 
 }  // extern "C"

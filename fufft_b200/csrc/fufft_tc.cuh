@@ -126,6 +126,11 @@ __device__ __forceinline__ bool elect()
    return p != 0;
 }
 
+__device__ __forceinline__ void arrive_own(uint64_t* bar)
+{
+   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(smem_u32(bar)) : "memory");
+}
+
 // ---- tiles on their way out ---------------------------------------------------
 // 2-D tile from shared memory; what lies outside the tensor is left out.  x, y not negative, x a multiple of 16 bytes
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* tm, int x, int y, const void* src)

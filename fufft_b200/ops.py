@@ -33,7 +33,7 @@ import torch
 
 from ._lib import (CACHE_MX4, CACHE_MX8, DTYPE_BF16, DTYPE_F16, DTYPE_F32, LAYOUT_NATURAL, LAYOUT_R8,
                    LAYOUT_R8_BPERM, LAYOUT_R16, LAYOUT_R16_BPERM, MID_CONJ_MULTIPLY, MID_MULTIPLY, MID_NONE,
-                   CacheDesc, FufftError, check, lib)
+                   MX4_DIRECT_ROWS, CacheDesc, FufftError, check, lib)
 
 __all__ = [
     "MID_NONE", "MID_MULTIPLY", "MID_CONJ_MULTIPLY",
@@ -593,9 +593,9 @@ def mx4_linear(x: torch.Tensor, w: Mx4, bias: torch.Tensor | None = None,
     dtype = dtype or x.dtype
     codes, out_code = _dtype(x.dtype), _dtype(dtype)
     out = flat.new_empty((m, w.rows), dtype=dtype)
-    q = _mx4_new(flat, m, k)
-    rc = lib().fufft_mx4_linear(flat.data_ptr(), codes, m, k, pitch, *q.at, *w.at, w.rows, _bias(bias, w.rows),
-                                out.data_ptr(), out_code, w.rows, _queue())
+    q = None if m <= MX4_DIRECT_ROWS else _mx4_new(flat, m, k)   # few rows are quantised inside the product
+    rc = lib().fufft_mx4_linear(flat.data_ptr(), codes, m, k, pitch, *(q.at if q else (None, None)), *w.at, w.rows,
+                                _bias(bias, w.rows), out.data_ptr(), out_code, w.rows, _queue())
     if rc:
         check(rc, "fufft_mx4_linear")
     return out if x.dim() == 2 else out.view(*x.shape[:-1], w.rows)

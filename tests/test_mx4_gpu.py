@@ -198,6 +198,27 @@ def test_linear(ops, dtype):
     assert bool(((got.cpu().double().view(6, 130) - want).abs() <= tol).all())
 
 
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(1, 130, 1), (1, 300, 31), (2, 64, 256), (5, 129, 257), (15, 200, 1000), (16, 4096, 4096), (16, 100, 40), (17, 100, 300)])
+def test_linear_few_rows(ops, shape, dtype):
+    """rows quantised inside the product: as those quantised before it, to the last bit, from any address, NaN and empty
+    blocks among them"""
+    m, n, k = shape
+    x = _values((m, k + 5), dtype, 7)
+    x[m // 2, (k - 1) // 2] = float("nan")
+    w = ops.mx4_quantize((torch.randn(n, k, generator=torch.Generator().manual_seed(8)) * 0.3).cuda())
+    bias = torch.randn(n, generator=torch.Generator().manual_seed(9)).cuda()
+    for off in (0, 1, 4):
+        d = x.cuda()[:, off:off + k]
+        for out in TYPES:
+            got = ops.mx4_linear(d, w, bias, dtype=out)
+            want = ops.mx4_matmul(ops.mx4_quantize(d), w, out, bias)
+            assert got.dtype == out
+            assert torch.equal(torch.nan_to_num(got, nan=7.0), torch.nan_to_num(want, nan=7.0))
+            assert torch.equal(torch.isnan(got), torch.isnan(want))
+
+
 GRADS = [(1, 1, 1), (5, 130, 70), (64, 96, 32), (130, 257, 300), (300, 65, 513)]
 
 
@@ -319,5 +340,8 @@ def test_refusals_before_device():
     assert L.fufft_mx4_matmul(P, P, None, P, None, P, 0, 4, 4, 64, 4, None) == ARG
     assert L.fufft_mx4_matmul(P, P + 4, P, P, None, P, 0, 4, 4, 64, 4, None) == MISALIGNED
     assert L.fufft_mx4_matmul(None, None, None, None, None, None, 0, 0, 4, 64, 4, None) == 0
+    linear = lambda m, x=P, c=P, stride=64, dtype=0: L.fufft_mx4_linear(x, dtype, m, 64, stride, c, c, P, P, 8, None, P, 0, 8, None)  # noqa: E731
+    assert linear(4, x=None) == ARG and linear(4, stride=63) == ARG and linear(4, dtype=3) == ARG and linear(4, x=P + 2) == MISALIGNED
+    assert linear(40, c=None) == ARG and linear(40, c=P + 8) == MISALIGNED and linear(0) == 0
     assert L.fufft_mx4_codes_bytes(3, 257) == 3 * 256 and L.fufft_mx4_scales_bytes(129, 1) == 2 * 2 * 512
     assert L.fufft_mx4_codes_bytes(-1, 4) == 0
