@@ -21,7 +21,7 @@ MID_NONE, MID_MULTIPLY, MID_CONJ_MULTIPLY = 0, 1, 2
 LAYOUT_R8, LAYOUT_R8_BPERM, LAYOUT_R16, LAYOUT_R16_BPERM, LAYOUT_NATURAL = 0, 1, 2, 3, 4
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
 CACHE_MX4, CACHE_MX8 = 0, 1
-MX4_DIRECT_ROWS = 16
+MX4_DIRECT_ROWS = 4
 
 # every symbol the header declares, with its C signature
 _P, _I, _I64, _U32 = ct.c_void_p, ct.c_int, ct.c_int64, ct.c_uint32

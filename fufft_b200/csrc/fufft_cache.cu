@@ -27,7 +27,8 @@ __device__ __forceinline__ int find_sequence(const int32_t* cu, int batch, long 
 // A CTA takes `per` tokens: their places are looked up once, by a thread each,
 // then its threads walk over the tokens' halves of blocks (16 channels, two
 // neighbouring lanes a block), a token after the other.  Bound by reading one
-// side and writing the other.
+// side and writing the other (65536 x 4096 bf16, MX4: append 106 us, read 109,
+// floor 104).
 constexpr int MAX_PER = 64;
 constexpr int THREADS = 256;
 
@@ -147,7 +148,8 @@ __global__ void __launch_bounds__(THREADS) read_kernel(T* __restrict__ out, long
 // brings sixteen channels of a position, a group of lanes takes a channel's
 // positions out, 16 bytes each.  The tile is skewed by 8 words per 16
 // channels: the lanes of a warp, 8 positions x 4 groups of channels, store
-// into 32 banks.
+// into 32 banks.  Bound by writing the rows, padding and all (8 x 4096 x 16384
+// fp32 from 8192 tokens MX4: 430 us, floor 349).
 constexpr int RN = 128, RC = 64, RPITCH = RN + 4;
 template<class T, bool MX8>
 __global__ void __launch_bounds__(THREADS) read_channels_kernel(T* __restrict__ out, Pages p,

@@ -32,14 +32,16 @@ struct MatmulArgs {
 // summed axis and join their sums through distributed shared memory, in rank
 // order.  Bound by reading b's codes and scales once.
 //
-// Rows that are not quantised yet (Raw<X>, sixteen at most) are quantised on
-// the way: two warps that have nothing else to do put each stage's 256 columns
+// Rows that are not quantised yet (Raw<X>, four at most) are quantised on the
+// way: two warps that have nothing else to do put each stage's 256 columns
 // into the layout that the copies would have left, in every CTA that needs
-// them; a launch and its wait less (one token 4096 x 4096: 7.5 us with the
-// quantiser's launch, 5.5 so).
+// them.  It saves a launch on the host (15.5 -> 9.6 us a call) and costs the
+// GPU nothing (us, inside / before: one token 4096 x 4096 5.8 / 6.7, 8192 x
+// 8192 8.1 / 8.7); sixteen rows would take the two warps longer than the
+// product (8192 x 8192 18.2 / 8.8).
 // ---------------------------------------------------------------------------
 struct Packed {};              // a comes in codes and scales
-template<class X> struct Raw {}; // a comes as rows of X
+template<class X> struct Raw {};   // a comes as rows of X
 struct RawArgs {
    const void* x;
    long long stride, cols;
@@ -62,31 +64,27 @@ template<int BN> struct Split {
    static_assert(STAGE % 1024 == 0, "the 128-byte swizzle repeats every 1024 bytes");
 };
 
-// A stage's columns of the unquantised rows, by 64 threads: a thread takes half
-// blocks of 16 values, two neighbouring lanes a block.
-template<class X>
-__device__ __forceinline__ void quantize_stage(const RawArgs& r, int rows, long long col0, uint8_t* codes, uint8_t* scales, int thread)
-{
-   Half<X> h[4];
-#pragma unroll
-   for(int u = 0; u < 4; ++u) {
-      const int row = u * 4 + (thread >> 4);
-      const long long col = col0 + (thread & 15) * HALF;
+// The unquantised rows, by 64 threads: a thread takes half a block of a stage,
+// two neighbouring lanes a block.  Four stages' loads are under way ahead of
+// the one that is encoded.
+template<class X> struct Turn {
+   Half<X> h;
+   __device__ __forceinline__ void load(const RawArgs& r, int rows, int row, long long col)
+   {
       const int count = row < rows ? (int)max(0ll, min((long long)HALF, r.cols - col)) : 0;
       const X* at = static_cast<const X*>(r.x) + row * r.stride + col;
-      if(r.on_32 && count == HALF) h[u].load(at);
-      else h[u].load_some(at, count);
+      if(r.on_32 && count == HALF) h.load(at);
+      else h.load_some(at, count);
    }
-#pragma unroll
-   for(int u = 0; u < 4; ++u) {
-      const int row = u * 4 + (thread >> 4), half = thread & 15;
+   __device__ __forceinline__ void store(uint8_t* codes, uint8_t* scales, int row, int half) const
+   {
       uint32_t q[2];
-      const uint32_t s = encode_pair<false>(h[u], q);
+      const uint32_t s = encode_pair<false>(h, q);
       // 128-byte rows whose 16-byte chunks are permuted by the row, as the copies' swizzle leaves them
       *reinterpret_cast<uint2*>(codes + row * 128 + ((half >> 1 ^ (row & 7)) << 4) + (half & 1) * 8) = make_uint2(q[0], q[1]);
       if((half & 1) == 0) scales[(half >> 3) * TILE_BYTES + tile_word(row) + (half >> 1 & 3)] = (uint8_t)s;
    }
-}
+};
 template<class A> struct RowType { using type = float; };
 template<class X> struct RowType<Raw<X>> { using type = X; };
 
@@ -96,7 +94,7 @@ __global__ void __launch_bounds__(128) matmul_split_kernel(const __grid_constant
 {
    using C = Split<BN>;
    constexpr bool PACKED = std::is_same_v<A, Packed>;
-   static_assert(PACKED || BN == 16, "sixteen rows at most are quantised here");
+   static_assert(PACKED || BN == 16, "four rows at most are quantised here");
    extern __shared__ uint8_t raw[];
    uint8_t* body = reinterpret_cast<uint8_t*>(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
    uint64_t* full = reinterpret_cast<uint64_t*>(body + C::BODY);
@@ -212,19 +210,29 @@ __global__ void __launch_bounds__(128) matmul_split_kernel(const __grid_constant
       }
       if(tc::elect()) tc::commit(done);
    } else if(!PACKED && warp >= 2) {
+      const int row = threadIdx.x >> 4 & 3, half = threadIdx.x & 15;
+      const long long col = (long long)k0 * K_PAD + half * HALF;
+      Turn<typename RowType<A>::type> ahead[4];
+#pragma unroll
+      for(int q = 0; q < 4; ++q)
+         if(q < n) ahead[q].load(x, (int)g.q_rows, row, col + (long long)q * K_PAD);
       int s = 0;
       uint32_t phase = 1;
-      for(int i = 0; i < n; ++i) {
-         if(!mbar_wait(empty + s, phase, g.status)) break;
-         uint8_t* at = body + s * C::STAGE + C::P_BYTES;
-         quantize_stage<typename RowType<A>::type>(x, (int)g.q_rows, (long long)(k0 + i) * K_PAD, at, at + C::Q_BYTES + C::SF_BYTES,
-                                                   threadIdx.x - 64);
-         fence_proxy_async_smem();
-         __syncwarp();
-         if(lane == 0) tc::arrive_own(full + s);
-         if(++s == C::STAGES) {
-            s = 0;
-            phase ^= 1;
+      bool ok = true;
+      for(int i = 0; i < n && ok; i += 4) {
+#pragma unroll
+         for(int q = 0; q < 4; ++q) {
+            if(i + q >= n || !(ok = mbar_wait(empty + s, phase, g.status))) break;
+            uint8_t* at = body + s * C::STAGE + C::P_BYTES;
+            ahead[q].store(at, at + C::Q_BYTES + C::SF_BYTES, row, half);
+            if(i + q + 4 < n) ahead[q].load(x, (int)g.q_rows, row, col + (long long)(i + q + 4) * K_PAD);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if(lane == 0) tc::arrive_own(full + s);
+            if(++s == C::STAGES) {
+               s = 0;
+               phase ^= 1;
+            }
          }
       }
    }

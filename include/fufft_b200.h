@@ -433,7 +433,7 @@ fufft_status fufft_mx4_matmul(const uint8_t* a_codes, const uint8_t* a_scales, c
  * quantize and w [n][k].  Up to FUFFT_MX4_DIRECT_ROWS rows are quantised on
  * the way, and x_codes / x_scales are not looked at (they may be NULL); beyond
  * that they are buffers of an m x k matrix and are left with Q(x). */
-#define FUFFT_MX4_DIRECT_ROWS 16
+#define FUFFT_MX4_DIRECT_ROWS 4
 fufft_status fufft_mx4_linear(const void* x, fufft_dtype x_dtype, int64_t m, int64_t k, int64_t x_stride,
                               uint8_t* x_codes, uint8_t* x_scales, const uint8_t* w_codes, const uint8_t* w_scales,
                               int64_t n, const float* bias, void* out, fufft_dtype dtype, int64_t out_stride,
