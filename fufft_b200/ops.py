@@ -419,9 +419,12 @@ _DTYPES = {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: D
 _raw_stream, _device_index = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
-def _queue() -> int:
-    """the current stream of the current device, as _stream, without making a stream object"""
-    return _raw_stream(_device_index())
+def _queue(t: torch.Tensor) -> int:
+    """the current stream of the current device, as _stream, without making a stream object; t has to be there"""
+    device = _device_index()
+    if t.get_device() != device:
+        raise ValueError(f"the tensors are on cuda:{t.get_device()}, the current device is cuda:{device}")
+    return _raw_stream(device)
 
 
 def _dtype(t: torch.dtype) -> int:
@@ -531,7 +534,7 @@ def mx4_quantize(x: torch.Tensor, transpose: bool = False) -> Mx4:
     else:
         q = _mx4_new(x, rows, cols)
         at = *q.at, None, None
-    rc = lib().fufft_mx4_quantize(x.data_ptr(), dtype, rows, cols, pitch, *at, _queue())
+    rc = lib().fufft_mx4_quantize(x.data_ptr(), dtype, rows, cols, pitch, *at, _queue(x))
     if rc:
         check(rc, "fufft_mx4_quantize")
     return q
@@ -544,7 +547,7 @@ def mx4_quantize_both(x: torch.Tensor) -> tuple[Mx4, Mx4]:
     rows, cols, pitch = _rows(x, "x")
     dtype = _dtype(x.dtype)
     q, qt = _mx4_new(x, rows, cols), _mx4_new(x, cols, rows)
-    rc = lib().fufft_mx4_quantize(x.data_ptr(), dtype, rows, cols, pitch, *q.at, *qt.at, _queue())
+    rc = lib().fufft_mx4_quantize(x.data_ptr(), dtype, rows, cols, pitch, *q.at, *qt.at, _queue(x))
     if rc:
         check(rc, "fufft_mx4_quantize")
     return q, qt
@@ -554,7 +557,7 @@ def mx4_dequantize(q: Mx4, dtype: torch.dtype = torch.float32, out: torch.Tensor
     """the values that q stands for"""
     code = _dtype(dtype)
     out, pitch = _result(out, q._buffer, q.rows, q.cols, dtype)
-    rc = lib().fufft_mx4_dequantize(*q.at, q.rows, q.cols, out.data_ptr(), code, pitch, _queue())
+    rc = lib().fufft_mx4_dequantize(*q.at, q.rows, q.cols, out.data_ptr(), code, pitch, _queue(out))
     if rc:
         check(rc, "fufft_mx4_dequantize")
     return out
@@ -575,7 +578,7 @@ def mx4_matmul(a: Mx4, b: Mx4, dtype: torch.dtype = torch.bfloat16, bias: torch.
     code = _dtype(dtype)
     out, pitch = _result(out, a._buffer, a.rows, b.rows, dtype)
     rc = lib().fufft_mx4_matmul(*a.at, *b.at, _bias(bias, b.rows), out.data_ptr(), code, a.rows, b.rows, a.cols, pitch,
-                                _queue())
+                                _queue(out))
     if rc:
         check(rc, "fufft_mx4_matmul")
     return out
@@ -595,7 +598,7 @@ def mx4_linear(x: torch.Tensor, w: Mx4, bias: torch.Tensor | None = None,
     out = flat.new_empty((m, w.rows), dtype=dtype)
     q = None if m <= MX4_DIRECT_ROWS else _mx4_new(flat, m, k)   # few rows are quantised inside the product
     rc = lib().fufft_mx4_linear(flat.data_ptr(), codes, m, k, pitch, *(q.at if q else (None, None)), *w.at, w.rows,
-                                _bias(bias, w.rows), out.data_ptr(), out_code, w.rows, _queue())
+                                _bias(bias, w.rows), out.data_ptr(), out_code, w.rows, _queue(out))
     if rc:
         check(rc, "fufft_mx4_linear")
     return out if x.dim() == 2 else out.view(*x.shape[:-1], w.rows)
@@ -660,7 +663,7 @@ def cache_append(cache: SeqCache, x: torch.Tensor, cu: torch.Tensor, starts: tor
     if channels != cache.channels:
         raise ValueError(f"x must have {cache.channels} channels")
     rc = lib().fufft_cache_append(cache.at, x.data_ptr(), _dtype(x.dtype), pitch, _i32(cu, cache.batch + 1, "cu"),
-                                  _i32(starts, cache.batch, "starts"), tokens, _queue())
+                                  _i32(starts, cache.batch, "starts"), tokens, _queue(x))
     if rc:
         check(rc, "fufft_cache_append")
 
@@ -673,7 +676,7 @@ def cache_read(cache: SeqCache, cu: torch.Tensor, starts: torch.Tensor, tokens: 
     if cache.batch == 0:
         out.zero_()
     rc = lib().fufft_cache_read(cache.at, out.data_ptr(), code, pitch, _i32(cu, cache.batch + 1, "cu"),
-                                _i32(starts, cache.batch, "starts"), tokens, _queue())
+                                _i32(starts, cache.batch, "starts"), tokens, _queue(out))
     if rc:
         check(rc, "fufft_cache_read")
     return out
@@ -687,7 +690,7 @@ def cache_read_channels(cache: SeqCache, starts: torch.Tensor, counts: torch.Ten
     code = _dtype(dtype)
     out = cache.codes.new_empty((cache.batch, cache.channels, n), dtype=dtype)
     rc = lib().fufft_cache_read_channels(cache.at, out.data_ptr(), code, n, _i32(starts, cache.batch, "starts"),
-                                         _i32(counts, cache.batch, "counts"), _queue())
+                                         _i32(counts, cache.batch, "counts"), _queue(out))
     if rc:
         check(rc, "fufft_cache_read_channels")
     return out
@@ -716,7 +719,7 @@ def cache_conv(cache: SeqCache, lengths: torch.Tensor, taps: torch.Tensor, gate:
             workspace = out.new_empty(need, dtype=torch.uint8)
     rc = lib().fufft_cache_conv(cache.at, _i32(lengths, cache.batch, "lengths"), taps.data_ptr(), _DTYPES[taps.dtype], n,
                                 heads, taps_pitch, gate_at, gate_pitch, out.data_ptr(), code, pitch, _ptr(workspace),
-                                0 if workspace is None else workspace.numel(), _queue())
+                                0 if workspace is None else workspace.numel(), _queue(out))
     if rc:
         check(rc, "fufft_cache_conv")
     return out
