@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(128) matmul_split_kernel(const __grid_constant
 // (tensor-memory lanes) are a's, and a warp hands tiles of 32 rows x 128 bytes
 // to tensor copies, where the rows of the result start on 16 bytes (8192 x
 // 4096 x 256 bf16, all of it storing: stores of whole sectors from the lanes
-// 29.6 us, the same without any 10.5); else the 256 rows are b's (SWAP), and
+// 29.6 us, tensor copies 14.3, no stores at all 10.5); else the 256 rows are b's (SWAP), and
 // the lanes of a warp store side by side, aligned or not.
 // ---------------------------------------------------------------------------
 template<int BN_, int ACC_> struct Pair {
@@ -660,8 +660,8 @@ template<class T> fufft_status matmul(const Operands& o, cudaStream_t st)
       return launch_split<T, 128>(o, split_for(tiles_p * ceil_div(o.m, 128), chunks, sms), ctx, st);
    if(chunks == 0) return launch_split<T, 128>(o, 1, ctx, st);
    // 256 columns in one accumulator or 192 in two of them, whichever covers the
-   // result in fewer columns' time (us, 256 / 192: 8192^3 189 / 195, 4096^3
-   // 30.9 / 28.5, 512 x 4096 x 4096 11.8 / 10.1)
+   // result in fewer columns' time (us, 256 / 192: 8192^3 189 / 201, 4096^3
+   // 28.1 / 26.7, 512 x 4096 x 4096 10.3 / 9.0)
    return ceil_div(wide, pairs) * 256 < ceil_div(narrow, pairs) * 192 ? launch_pair<T, Pair<256, 1>>(o, ctx, st)
                                                                      : launch_pair<T, Pair<192, 2>>(o, ctx, st);
 }
