@@ -20,6 +20,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "fufft_internal.cuh"
 
 namespace fufft {
@@ -100,26 +102,47 @@ __device__ __forceinline__ void store32(void* p, const uint32_t* w)
 // a NaN above an infinity, so an integer maximum keeps both
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-// maximum of abs_bits over N values as they lie in memory, three words an
-// instruction; of 16-bit values two maxima, in the halves of a word
+// |x| as bits of the largest of N values as they lie in memory, three words an
+// instruction; of 16-bit values two maxima, in the halves of a word.  The
+// signed maximum is the largest of those without a sign bit, the unsigned one
+// the largest of those with it (if there are any): no bit has to be masked on
+// the way.  fp32 has an instruction for the maximum of magnitudes that keeps NaN.
 template<class T, int N> __device__ __forceinline__ uint32_t max_words(const uint32_t* w)
 {
-   constexpr uint32_t MASK = sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu;
-   uint32_t m = w[0] & MASK;
+   static_assert(N % 2 == 0, "the first, pairs, the last");
+   if constexpr(sizeof(T) == 4) {
+      float m = __uint_as_float(w[0]);
 #pragma unroll
-   for(int i = 1; i + 1 < N; i += 2) {
-      if constexpr(sizeof(T) == 4) m = __vimax3_u32(m, w[i] & MASK, w[i + 1] & MASK);
-      else m = __vimax3_u16x2(m, w[i] & MASK, w[i + 1] & MASK);
+      for(int i = 1; i + 1 < N; i += 2)
+         asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(__uint_as_float(w[i])), "f"(__uint_as_float(w[i + 1])));
+      asm("max.NaN.abs.f32 %0, %0, %1, %1;" : "+f"(m) : "f"(__uint_as_float(w[N - 1])));
+      return __float_as_uint(m) & 0x7fffffffu;
+   } else {
+      uint32_t p = w[0], n = w[0];
+#pragma unroll
+      for(int i = 1; i + 1 < N; i += 2) {
+         p = __vimax3_s16x2(p, w[i], w[i + 1]);
+         n = __vimax3_u16x2(n, w[i], w[i + 1]);
+      }
+      p = __vimax3_s16x2(p, p, w[N - 1]);
+      n = __vimax3_u16x2(n, n, w[N - 1]);
+      return __vimax3_s16x2(p, p, n & 0x7fff7fffu);
    }
-   if constexpr(sizeof(T) == 4) return max(m, w[N - 1] & MASK);
-   else return __vimax3_u16x2(m, m, w[N - 1] & MASK);
 }
-// values v[2 i], v[2 i + 1] = those of w[i] times a power of two
-template<class T> __device__ __forceinline__ void scaled_pair(uint32_t w, float factor, float* v)
+// the two values of w, each times its power of two.  A bfloat16 holds every
+// power of two that scale_inverse returns, and one mixed fma widens and
+// multiplies a half, exactly; minus zero is what keeps the sign of a zero
+template<class T> __device__ __forceinline__ void scaled_pair(uint32_t w, float2 factor, float* a, float* b)
 {
-   const float2 f = fmul2(unpack2<T>(w), make_float2(factor, factor));
-   v[0] = f.x;
-   v[1] = f.y;
+   if constexpr(std::is_same<T, __nv_bfloat16>::value) {
+      asm("{\n\t.reg .b16 lo, hi, f0, f1, z;\n\tmov.b32 {lo, hi}, %2;\n\tmov.b32 {z, f0}, %3;\n\tmov.b32 {z, f1}, %4;\n\t"
+          "fma.rn.f32.bf16 %0, lo, f0, %5;\n\tfma.rn.f32.bf16 %1, hi, f1, %5;\n\t}"
+          : "=f"(*a), "=f"(*b) : "r"(w), "r"(__float_as_uint(factor.x)), "r"(__float_as_uint(factor.y)), "f"(-0.0f));
+   } else {
+      const float2 f = fmul2(unpack2<T>(w), factor);
+      *a = f.x;
+      *b = f.y;
+   }
 }
 
 // Sixteen consecutive values as they lie in memory: half a block, the unit of
@@ -187,7 +210,7 @@ template<class T> struct Half {
             v[2 * i] = f.x;
             v[2 * i + 1] = f.y;
          } else {
-            scaled_pair<T>(w[i], factor, v + 2 * i);
+            scaled_pair<T>(w[i], make_float2(factor, factor), v + 2 * i, v + 2 * i + 1);
          }
       }
    }
@@ -207,8 +230,8 @@ template<int EMAX> __device__ __forceinline__ uint32_t scale_byte(uint32_t max_b
    const int e = (int)(max_bits >> 23);
    return e == 255 ? 255u : (uint32_t)max(e - EMAX, 0);
 }
-// 2^(127 - s); 0 for a NaN block, so that its codes are zero
-__device__ __forceinline__ float scale_inverse(uint32_t s) { return s == 255u ? 0.0f : __uint_as_float((254u - s) << 23); }
+// 2^(127 - s) (s <= 252, or a NaN block's, for which any will do)
+__device__ __forceinline__ float scale_inverse(uint32_t s) { return __uint_as_float((254u - s) << 23); }
 // 2^(s - 127); NaN for s = 255
 __device__ __forceinline__ float scale_value(uint32_t s)
 {
@@ -316,11 +339,11 @@ template<bool MX8, class T> __device__ __forceinline__ uint32_t encode_pair(cons
    const float inv = scale_inverse(s);
    float v[HALF];
    h.scaled(inv, v);
+   Elem<MX8>::encode(v, w);
    if(s == 255u) {   // zero codes under a NaN scale
 #pragma unroll
-      for(int i = 0; i < HALF; ++i) v[i] = 0.0f;
+      for(int i = 0; i < Elem<MX8>::WORDS; ++i) w[i] = 0;
    }
-   Elem<MX8>::encode(v, w);
    return s;
 }
 

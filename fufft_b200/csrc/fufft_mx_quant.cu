@@ -42,8 +42,8 @@ template<class T> bool rows_on_32(const void* p, long long row_stride)
 
 // Rows: a warp takes U x 512 columns of a row, a lane sixteen of each, two
 // lanes a block, eight lanes the four blocks of a scale word.  Columns beyond
-// `cols` are zeros.  Bound by reading x and writing the codes (16384^2 bf16 104
-// us, its floor; 8192^2 fp32 46).
+// `cols` are zeros.  Bound by reading x and writing the codes (16384^2 bf16 98
+// us, floor 104; 8192^2 fp32 46).
 constexpr int SPAN = 32 * HALF;   // columns of a warp's pass
 constexpr int STAGE = SPAN + SPAN / HALF;
 
@@ -112,9 +112,11 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict_
 // apart, next to the other lanes' groups (place, word_at), and every 32 rows
 // are skewed by 8 words: both the stores of the rows and the loads of 8 words
 // x 4 blocks fall on 32 banks.
-// Bound by the reads and writes with fp32 (8192^2 both ways 65 us, floor 52; two
-// CTAs an SM, whose registers hold a block, beat three, 78), by the ALU and the
-// phases of a tile with 16 bits (46 us, floor 31; two CTAs 55).
+// Bound by the reads and writes with fp32 (8192^2 both ways 61 us, floor 52; two
+// CTAs an SM, whose registers hold a block: 65 before the maxima took abs values
+// unmasked, then three 78), by the ALU and the phases of a tile with bfloat16
+// (40 us, floor 31; four CTAs the same; 46 while halves were widened by masks
+// and shifts and zeroed one by one, then two 55).
 constexpr int QT = 128;
 template<class T> struct Tile {
    static constexpr int PITCH = QT * (int)sizeof(T) / 4 + 4;         // words; rows stay on 16 bytes
@@ -134,14 +136,11 @@ template<class T> struct Tile {
    }
 };
 
-// 32 values over the block's scale -> its sixteen bytes of codes
-__device__ __forceinline__ uint4 encode_block(uint32_t s, float* v)
+// 32 values over the block's scale -> its sixteen bytes of codes, zeros under a NaN scale
+__device__ __forceinline__ uint4 encode_block(uint32_t s, const float* v)
 {
-   if(s == 255u) {
-#pragma unroll
-      for(int i = 0; i < BLOCK; ++i) v[i] = 0.0f;
-   }
-   return make_uint4(e2m1_encode8(v), e2m1_encode8(v + 8), e2m1_encode8(v + 16), e2m1_encode8(v + 24));
+   const uint4 q = make_uint4(e2m1_encode8(v), e2m1_encode8(v + 8), e2m1_encode8(v + 16), e2m1_encode8(v + 24));
+   return s == 255u ? make_uint4(0, 0, 0, 0) : q;
 }
 
 template<class T, bool ROWS>
@@ -239,9 +238,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) quantize_tile_ker
          float v1[BLOCK];
 #pragma unroll
          for(int i = 0; i < BLOCK; ++i) {
-            const float2 f = fmul2(unpack2<T>(raw[i]), inv);
-            v[i] = f.x;
-            v1[i] = f.y;
+            scaled_pair<T>(raw[i], inv, v + i, v1 + i);
          }
          q[0] = encode_block(s[0], v);
          q[1] = encode_block(s[1], v1);
@@ -309,7 +306,7 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restri
 }
 
 // four passes a warp in flight where rows have them and the card stays full;
-// else one (16 x 4096 bf16: 2.2 us against 2.9, 8192^2 34.6 against 56)
+// else one (bf16, one / four: 16 x 4096 2.1 / 2.7 us, 16384^2 112 / 98)
 bool four_passes(long long rows, long long spans) { return spans >= 4 && rows * spans >= 32 * 148; }
 
 template<class T>
