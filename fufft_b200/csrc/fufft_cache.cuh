@@ -33,9 +33,10 @@ struct Pages {
       if(pos < 0 || pos > 0x7fffffffll) return -1;
       const unsigned k = (unsigned)pos / (unsigned)page_size;
       if(k >= (unsigned)max_pages) return -1;
-      const int page = __ldg(table + b * table_stride + k);
-      return page < 0 || page >= pages ? -1 : page * page_size + (int)((unsigned)pos - k * (unsigned)page_size);
+      return row(__ldg(table + b * table_stride + k), (int)((unsigned)pos - k * (unsigned)page_size));
    }
+   // position `in` of a page of the table, or -1 where there is no such page
+   __device__ __forceinline__ int row(int page, int in) const { return page < 0 || page >= pages ? -1 : page * page_size + in; }
 };
 
 fufft_status check_cache(const fufft_cache* c);

@@ -128,10 +128,11 @@ __device__ __forceinline__ void park(float* joined, const float2 (&acc)[NB][CH /
 
 // Adds the slots of this CTA in their order, then the CTAs of its cluster in
 // theirs (through distributed shared memory, a part of the results each), and
-// writes the results, or the cluster's part of them where there are several.
+// writes the results, or the cluster's part of them where there are several
+// (rows `part`, one a sequence).
 template<int NB>
 __device__ __forceinline__ void join(float* joined, const ConvStep& a, const Pages& p, int width, int slots, int threads,
-                                     int rank, int b0, int c0)
+                                     int rank, int b0, int c0, long long part)
 {
    __syncthreads();
    for(int e = threadIdx.x; e < NB * width; e += threads) {
@@ -155,7 +156,7 @@ __device__ __forceinline__ void join(float* joined, const ConvStep& a, const Pag
 #pragma unroll
          for(int r = 0; r < MAX_SPLIT; ++r) y += v[r];
       }
-      if(a.partial) a.partial[((long long)(blockIdx.x / a.split) * p.batch + b0 + s) * a.channels + c0 + i] = y;
+      if(a.partial) a.partial[(part + s) * a.channels + c0 + i] = y;
       else finish(a, b0 + s, c0 + i, y);
    }
    if(a.split > 1) tc::cluster_sync();   // nobody leaves while its sums are being read
@@ -239,7 +240,7 @@ __global__ void __launch_bounds__(THREADS, 2) conv_step_kernel(Pages p, ConvStep
    }
 
    if(slot < a.slots) park<NB>(joined, acc, slot, lane, a.slots, a.lanes);
-   join<NB>(joined, a, p, a.lanes * CH, a.slots, THREADS, rank, b0, c0);
+   join<NB>(joined, a, p, a.lanes * CH, a.slots, THREADS, rank, b0, c0, (long long)(blockIdx.x / a.split) * p.batch + b0);
 }
 
 // joins the clusters in their order
@@ -260,15 +261,22 @@ __global__ void __launch_bounds__(256) conv_join_kernel(ConvStep a, int batch)
 // four rows each; a row that is not there is one outside the tensor, and reads
 // as zeros), the taps (one tensor copy, 16-byte chunks permuted so that the
 // lanes' wide loads fall on different banks) and the scales, with the taps that
-// heads share.  A warp fills each slot of the ring.  Eight warps sum: a thread keeps 16
-// channels of the NS sequences, so a tap is widened once for all of them.
+// heads share.  A warp fills each slot of the ring; it asks for the pages and
+// the scales a stage ahead.  Eight warps sum: a thread keeps 16 channels of the
+// NS sequences, so a tap is widened once for all of them.
 //
 // Two ways to sum a value.  Where every scale of the stage is a half-precision
-// number (2^-24 .. 2^15) and every row is there, an exact fma widens the half
-// x and scales it, one instruction on both halves of the FMA pipe, and half a
-// packed fma adds it times its tap: twice as fast as the general way, whose
-// widening and packed product and sum all go to one half of the pipe (B200, a
-// loop of them alone: 29 values a clock and SM).
+// number (2^-24 .. 2^15), an exact fma widens the half x and scales it, one
+// instruction on both halves of the FMA pipe, and half a packed fma adds it
+// times its tap: twice as fast as the general way, whose widening and packed
+// product and sum all go to one half of the pipe (B200, a loop of them alone:
+// 29 values a clock and SM, 49 this way).  Where rows are missing, each row is
+// asked for first (16 sequences of 16384 to 32768, one empty, x 2048 MX4: 171
+// us; 201 where such stages took the general way).
+// 16 x 32768 x 2048 MX4, bf16 taps: 200 us, floor 107; the sums alone, without
+// a ring to wait for, 165 (130 with taps that heads share, which are read and
+// widened once a block).  Sixteen warps of eight channels a thread: the sums
+// alone 171, with the ring 212.
 // ---------------------------------------------------------------------------
 namespace pipe {
 constexpr int CONSUMERS = 8, PRODUCERS = 4, THREADS = (CONSUMERS + PRODUCERS) * 32;   // warps that sum; that fill
@@ -281,8 +289,92 @@ struct Args {
    int lags, stages, stage_bytes, codes_at, scales_at;   // of a stage: lags; offsets of its parts (taps at 0)
    int row_bytes;                                        // of the CTA's chunk
    int tap_bytes;                                        // of a lag's taps in the chunk
+   int pool;                                             // CTAs of a chunk that the lags are dealt to, or 0
    bool quads;                                           // four blocks' scales at once
 };
+
+// Long histories of unequal lengths: the stages of all groups of NS sequences
+// are dealt to `pool` CTAs, each of one group, by one warp, to
+// starts[group] .. starts[group + 1] - 1: with q the least number for which
+// sum ceil(stages of a group / q) does not exceed the pool, a group of t
+// stages gets ceil(t / q) CTAs.  pool is at least twice the groups.
+constexpr int MAX_GROUPS = 128;
+__device__ __forceinline__ int upper_bound(const int* starts, int groups, int worker)   // the group of a CTA; `groups` beyond the last
+{
+   int lo = 0, hi = groups;
+   while(lo < hi) {
+      const int mid = (lo + hi) / 2;
+      if(starts[mid + 1] > worker) hi = mid;
+      else lo = mid + 1;
+   }
+   return lo;
+}
+template<int NS> __device__ __noinline__ void deal(const int32_t* lengths, int batch, int n_taps, int lags, int pool, int lane, int* starts)
+{
+   const int groups = (batch + NS - 1) / NS;
+   int t[MAX_GROUPS / 32];
+   long long total = 0;
+#pragma unroll
+   for(int k = 0; k < MAX_GROUPS / 32; ++k) {
+      int longest = 0;
+      for(int s = 0; s < NS; ++s) {
+         const int b = (k * 32 + lane) * NS + s;
+         if(b < batch) longest = max(longest, lengths[b]);
+      }
+      t[k] = (int)(((unsigned)min(longest, n_taps) + lags - 1) / (unsigned)lags);
+      total += t[k];
+   }
+#pragma unroll
+   for(int d = 16; d; d /= 2) total += __shfl_xor_sync(0xffffffffu, total, d);
+   int lo = max(1, (int)((total + pool - 1) / pool)), hi = max(1, (int)((total + pool - groups - 1) / (pool - groups)));
+   while(lo < hi) {
+      const int mid = lo + (hi - lo) / 2;
+      int need = 0;
+#pragma unroll
+      for(int k = 0; k < MAX_GROUPS / 32; ++k) need += (t[k] + mid - 1) / mid;
+      if((int)__reduce_add_sync(0xffffffffu, need) <= pool) hi = mid;
+      else lo = mid + 1;
+   }
+   int before = 0;
+   if(lane == 0) starts[0] = 0;
+#pragma unroll
+   for(int k = 0; k < MAX_GROUPS / 32; ++k) {
+      int sum = (t[k] + lo - 1) / lo;
+#pragma unroll
+      for(int d = 1; d < 32; d *= 2) {
+         const int other = __shfl_up_sync(0xffffffffu, sum, d);
+         if(lane >= d) sum += other;
+      }
+      if(k * 32 + lane < groups) starts[k * 32 + lane + 1] = before + sum;
+      before += __shfl_sync(0xffffffffu, sum, 31);
+   }
+}
+
+// a CTA's share: its first sequence, its number among the CTAs of the group
+// and theirs, the longest history within the taps, its stages
+struct Share {
+   int b0, worker, workers, longest, n;
+};
+// the length of sequence lane % NS of a group
+template<int NS> __device__ __forceinline__ int b_length(const ConvStep& a, const Pages& p, int b0, int lane)
+{
+   return b0 + lane % NS < p.batch ? max(a.lengths[b0 + lane % NS], 0) : 0;
+}
+
+// joins the CTAs of a sequence's group, in their order
+template<int NS>
+__global__ void __launch_bounds__(256) join_dealt_kernel(ConvStep a, int batch, int lags, int pool)
+{
+   __shared__ int starts[MAX_GROUPS + 1];
+   if(threadIdx.x < 32) deal<NS>(a.lengths, batch, a.n_taps, lags, pool, threadIdx.x, starts);
+   __syncthreads();
+   const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+   if(i >= (long long)batch * a.channels) return;
+   const int b = (int)(i / a.channels), c = (int)(i % a.channels);
+   float y = 0.0f;
+   for(int w = starts[b / NS]; w < starts[b / NS + 1]; ++w) y += a.partial[((long long)w * NS + b % NS) * a.channels + c];
+   finish(a, b, c, y);
+}
 
 __device__ __forceinline__ void load_taps(const CUtensorMap* tm, void* dst, int x, int y, int z, uint64_t* bar)
 {
@@ -314,23 +406,44 @@ __device__ __forceinline__ uint32_t scale_entry(uint32_t s)
    return half | s << 16 | (half ? 0u : NO_HALF);
 }
 
-// cache rows of the pairs (lag, sequence) of a stage, pair = lag * NS + sequence; -1 without one
-template<int NS>
-__device__ __forceinline__ void find_rows(const Pages& p, int b0, int len, int lane, int pairs, int filled, long long j0, int* rows)
-{
-   __syncwarp();
-   for(int pair = lane; pair < filled; pair += 32) {   // a lane's sequence, lane % NS, is the same throughout
-      const long long j = j0 + pair / NS;
-      rows[pair] = pair < pairs && j < len ? p.slot(b0 + lane % NS, (long long)len - 1 - j) : -1;
+// Cache rows of the pairs (lag, sequence) of a stage, pair = lag * NS +
+// sequence; -1 without one.  For the first 64 the page table is asked a stage
+// ahead of the use.  Loads that are ahead of their use have no condition (a
+// lane without a pair reads any entry): what a branch may or may not have
+// loaded is waited for where the branch ends.
+template<int NS> struct Rows {
+   static constexpr int AHEAD = 2;
+   int page[AHEAD], in[AHEAD];
+   __device__ __forceinline__ void ask(const Pages& p, int b0, int len, int lane, int pairs, long long j0)
+   {
+#pragma unroll
+      for(int k = 0; k < AHEAD; ++k) {
+         const int pair = k * 32 + lane;   // a lane's sequence, lane % NS, is the same throughout
+         const long long pos = len - 1 - (j0 + pair / NS);
+         const unsigned at = (unsigned)max(0ll, pos) / (unsigned)p.page_size;
+         const bool there = pair < pairs && pos >= 0 && at < (unsigned)p.max_pages;
+         in[k] = there ? (int)((unsigned)pos - at * (unsigned)p.page_size) : -1;
+         page[k] = __ldg(p.table + (there ? (b0 + lane % NS) * p.table_stride + at : 0));
+      }
    }
-   __syncwarp();
-}
+   __device__ __forceinline__ void settle(const Pages& p, int b0, int len, int lane, int pairs, int filled, long long j0, int* rows) const
+   {
+      __syncwarp();
+#pragma unroll
+      for(int k = 0; k < AHEAD; ++k)
+         if(k * 32 + lane < filled) rows[k * 32 + lane] = in[k] < 0 ? -1 : p.row(page[k], in[k]);
+      for(int pair = AHEAD * 32 + lane; pair < filled; pair += 32) {
+         const long long j = j0 + pair / NS;
+         rows[pair] = pair < pairs && j < len ? p.slot(b0 + lane % NS, len - 1 - j) : -1;
+      }
+      __syncwarp();
+   }
+};
 
-// The scales of a stage, [pair][block]: a lane takes W blocks of a row, eight
-// rows a batch.  The first batch is loaded before the stage is known to be
-// free, and put there when it is.
-template<int W> struct Scales {
-   static constexpr int BATCH = 8;
+// The scales of a stage, [pair][block]: a lane takes W blocks of a row, BATCH
+// rows at a time.  The first batch is loaded a stage ahead, and put into place
+// when the slot is free.
+template<int W, int BATCH> struct Scales {
    int each, at_once, mine, b0;   // 2^each lanes a row, rows at a time, this lane's row and its first block
    uint32_t raw[BATCH];
    int row[BATCH];
@@ -348,11 +461,9 @@ template<int W> struct Scales {
       for(int k = 0; k < BATCH; ++k) {
          const int pair = first + k * at_once + mine;
          row[k] = pair < pairs && b < blocks ? rows[pair] : -2;
-         if(row[k] >= 0) {
-            const uint8_t* at = scales + (long long)row[k] * row_scales + b;
-            if constexpr(W == 4) raw[k] = __ldg(reinterpret_cast<const unsigned int*>(at));
-            else raw[k] = __ldg(at);
-         }
+         const uint8_t* at = scales + (row[k] < 0 ? 0 : (long long)row[k] * row_scales + b);   // no condition: nothing to wait for
+         if constexpr(W == 4) raw[k] = __ldg(reinterpret_cast<const unsigned int*>(at));
+         else raw[k] = __ldg(at);
       }
    }
    // the entries' flags
@@ -390,7 +501,7 @@ template<int W> struct Scales {
    }
 };
 
-// The taps of a stage that blocks share, [lag][block], as numbers; eight loads under way.
+// The taps of a stage that blocks share, [lag][block], as numbers; sixteen loads under way.
 template<class TT>
 __device__ __forceinline__ void stage_taps(const TT* taps, long long stride, int c0, int group, float* out, int pitch, int blocks,
                                            int lags, int lane)
@@ -398,19 +509,20 @@ __device__ __forceinline__ void stage_taps(const TT* taps, long long stride, int
    const int each = blocks <= 1 ? 0 : min(5, 32 - __clz(blocks - 1)), at_once = 32 >> each, mine = lane >> each;
    for(int b = lane & ((1 << each) - 1); b < blocks; b += 1 << each) {
       const int head = (c0 + b * mx::BLOCK) / group;
-      for(int first = mine; first < lags; first += 8 * at_once) {
-         TT t[8];
+      for(int first = mine; first < lags; first += 16 * at_once) {
+         TT t[16];
 #pragma unroll
-         for(int k = 0; k < 8; ++k)
+         for(int k = 0; k < 16; ++k)
             if(first + k * at_once < lags) t[k] = taps[(first + k * at_once) * stride + head];
 #pragma unroll
-         for(int k = 0; k < 8; ++k)
+         for(int k = 0; k < 16; ++k)
             if(first + k * at_once < lags) out[(first + k * at_once) * pitch + b] = mx::to_f(t[k]);
       }
    }
 }
 
-// What a consumer does with its lags of a stage.  FAST: every scale a half, every row there.
+// What a consumer does with its lags of a stage.  FAST: every scale a half; ALL: every row there too.
+enum class Sum { ALL, FAST, ANY };
 template<bool MX8, class TT, bool HEAD, int NB> struct Lag {   // what a thread reads of one lag
    uint32_t q[NB][MX8 ? 4 : 2], e[NB], t[HEAD ? 1 : CH * sizeof(TT) / 4];
    __device__ __forceinline__ void load(const uint8_t* at, uint32_t off, const uint8_t* codes, int row, const uint32_t* scales, int blocks)
@@ -443,20 +555,21 @@ template<bool MX8, class TT, bool HEAD, int NB> struct Lag {   // what a thread 
       else if constexpr(sizeof(TT) == 4) return make_float2(__uint_as_float(t[2 * k]), __uint_as_float(t[2 * k + 1]));
       else return mx::unpack2<__nv_bfloat16>(t[k]);
    }
-   template<bool FAST> __device__ __forceinline__ void sum(float2 (&acc)[NB][CH / 2]) const
+   template<Sum HOW> __device__ __forceinline__ void sum(float2 (&acc)[NB][CH / 2]) const
    {
       float2 w[HEAD ? 1 : CH / 2];
 #pragma unroll
       for(int k = 0; k < (HEAD ? 1 : CH / 2); ++k) w[k] = tap(k);
 #pragma unroll
       for(int s = 0; s < NB; ++s) {
+         if constexpr(HOW != Sum::ALL)
+            if(e[s] & NO_ROW) continue;   // nothing, whatever the tap is
          uint32_t v[CH / 2];
          mx::Elem<MX8>::halves(q[s], v);
-         if constexpr(FAST) {
+         if constexpr(HOW != Sum::ANY) {
 #pragma unroll
             for(int k = 0; k < CH / 2; ++k) acc[s][k] = ffma2(widen_scaled(v[k], e[s]), w[HEAD ? 0 : k], acc[s][k]);
          } else {
-            if(e[s] & NO_ROW) continue;
             const float scale = mx::scale_value(e[s] >> 16 & 255);
 #pragma unroll
             for(int k = 0; k < CH / 2; ++k) acc[s][k] = ffma2(fmul2(mx::half2_f(v[k]), make_float2(scale, scale)), w[HEAD ? 0 : k], acc[s][k]);
@@ -469,7 +582,7 @@ struct Path {
    uint32_t tap, tap_step;
    int codes, codes_step, row, scales, scales_step, blocks, slot, slots;
 };
-template<bool MX8, class TT, bool HEAD, int NB, bool FAST>
+template<bool MX8, class TT, bool HEAD, int NB, Sum HOW>
 __device__ __forceinline__ void sum_stage(const uint8_t* at, const Path& w, int count, float2 (&acc)[NB][CH / 2])
 {
    using L = Lag<MX8, TT, HEAD, NB>;
@@ -480,28 +593,39 @@ __device__ __forceinline__ void sum_stage(const uint8_t* at, const Path& w, int 
    for(int l = w.slot; l < count; l += w.slots, tap += w.tap_step, codes += w.codes_step, scales += w.scales_step) {
       L one;
       one.load(at, tap, codes, w.row, scales, w.blocks);
-      one.template sum<FAST>(acc);
+      one.template sum<HOW>(acc);
    }
 }
 
 template<class TT, bool HEAD, int NS, int W>
 __device__ __forceinline__ void fill(const CUtensorMap* codes_map, const CUtensorMap* taps_map, const Pages& p, const Args& g, uint8_t* ring,
-                                     uint64_t* full, uint64_t* empty, uint32_t* flags, const uint32_t* entry, int* found, int st, int n,
-                                     int worker, int workers, int longest, int mine, int b0, int c0, int x, int blocks, int lane)
+                                     uint64_t* full, uint64_t* empty, uint32_t* flags, const uint32_t* entry, int* found, int st,
+                                     const Share share, int mine, int c0, int x, int blocks, int lane)
 {
    const ConvStep& a = g.a;
    uint8_t* at = ring + st * g.stage_bytes;
    uint32_t* out = reinterpret_cast<uint32_t*>(at + g.scales_at);
    const uint8_t* scales = p.scales + c0 / mx::BLOCK;
    const int row_scales = a.channels / mx::BLOCK;
-   Scales<W> sc(blocks, lane);
+   Scales<W, HEAD ? 16 : 8> sc(blocks, lane);
    uint32_t phase = 1;
    bool ok = true;
-   for(int i = st; i < n; i += g.stages, phase ^= 1) {
-      const long long j0 = (long long)(worker + (long long)i * workers) * g.lags;
-      const int count = (int)min((long long)g.lags, longest - j0);
-      find_rows<NS>(p, b0, mine, lane, count * NS, g.lags * NS, j0, found);
-      sc.load(found, scales, row_scales, 0, sc.b0, blocks, count * NS);
+   const auto first = [&](long long i) { return (share.worker + i * share.workers) * g.lags; };   // lag of stage i
+   const auto held = [&](long long j0) { return (int)max(0ll, min((long long)g.lags, share.longest - j0)); };
+   Rows<NS> next;
+   const auto ask = [&](long long j0) { next.ask(p, share.b0, mine, lane, held(j0) * NS, j0); };
+   // the rows of the stage whose pages were asked for, and its scales; the pages of the one after it
+   const auto look_ahead = [&](long long i) {
+      const long long j0 = first(i);
+      next.settle(p, share.b0, mine, lane, held(j0) * NS, g.lags * NS, j0, found);
+      sc.load(found, scales, row_scales, 0, sc.b0, blocks, held(j0) * NS);
+      ask(first(i + g.stages));
+   };
+   ask(first(st));
+   look_ahead(st);
+   for(int i = st; i < share.n; i += g.stages, phase ^= 1) {
+      const long long j0 = first(i);
+      const int count = held(j0);
       if(!(ok = mbar_wait(empty + st, phase, g.status))) break;
       if(tc::elect()) {
          mbar_expect_tx(full + st, g.lags * (NS * g.row_bytes + (HEAD ? 0 : g.tap_bytes)));
@@ -520,6 +644,7 @@ __device__ __forceinline__ void fill(const CUtensorMap* codes_map, const CUtenso
       if(lane == 0) flags[st] = seen | (uint32_t)count;
       __syncwarp();
       if(lane == 0) tc::arrive_own(full + st);
+      look_ahead((long long)i + g.stages);
    }
    if(!ok) {   // a wait gave up: time for the copies under way to land
       const uint64_t t0 = globaltimer_ns();
@@ -537,17 +662,13 @@ __global__ void __launch_bounds__(THREADS, 1) conv_pipe_kernel(const __grid_cons
    __shared__ uint64_t full[MAX_STAGES], empty[MAX_STAGES];
    __shared__ uint32_t flags[MAX_STAGES], entry[256];   // lags of a stage, with NO_HALF and NO_ROW where one of its scales has it
    __shared__ __align__(16) int rows[PRODUCERS][MAX_PAIRS];
+   __shared__ int starts[MAX_GROUPS + 1];
+   __shared__ Share share;
    const ConvStep& a = g.a;
    const int warp = tc::uniform_warp(), lane = threadIdx.x & 31;
    const int rank = a.split > 1 ? (int)tc::cluster_rank() : 0;
-   const int worker = blockIdx.x, workers = a.split * a.outer;
-   const int c0 = blockIdx.y * a.lanes * CH, b0 = blockIdx.z * NS;
+   const int c0 = blockIdx.y * a.lanes * CH;
    const int units = min(a.lanes, a.channels / CH - (int)blockIdx.y * a.lanes), blocks = units / 2;
-
-   // the length of sequence lane % NS, and the longest of the NS, within the taps
-   const int mine = b0 + lane % NS < p.batch ? max(a.lengths[b0 + lane % NS], 0) : 0;
-   const int longest = min((int)__reduce_max_sync(0xffffffffu, (unsigned)mine), a.n_taps);
-   const int tiles = (int)(((long long)longest + g.lags - 1) / g.lags), n = tiles > worker ? (tiles - 1 - worker) / workers + 1 : 0;
    if(threadIdx.x == 0) {
       for(int s = 0; s < g.stages; ++s) {
          mbar_init(full + s, 2);
@@ -558,7 +679,31 @@ __global__ void __launch_bounds__(THREADS, 1) conv_pipe_kernel(const __grid_cons
       if(!HEAD) prefetch_tmap(&taps_map);
    }
    if(threadIdx.x < 256) entry[threadIdx.x] = scale_entry(threadIdx.x);
+   if(warp == CONSUMERS) {   // what this CTA does
+      Share w{(int)blockIdx.z * NS, (int)blockIdx.x, a.split, 0, 0};
+      if(g.pool) {
+         const int groups = (p.batch + NS - 1) / NS;
+         deal<NS>(a.lengths, p.batch, a.n_taps, g.lags, g.pool, lane, starts);
+         __syncwarp();
+         const int group = upper_bound(starts, groups, w.worker);
+         if(group < groups) {
+            w.b0 = group * NS;
+            w.workers = starts[group + 1] - starts[group];
+            w.worker -= starts[group];
+         } else {
+            w.b0 = -1;
+         }
+      }
+      if(w.b0 >= 0) {
+         const int mine = b_length<NS>(a, p, w.b0, lane);
+         w.longest = min((int)__reduce_max_sync(0xffffffffu, (unsigned)mine), a.n_taps);
+         const int tiles = (int)(((long long)w.longest + g.lags - 1) / g.lags);
+         w.n = tiles > w.worker ? (tiles - 1 - w.worker) / w.workers + 1 : 0;
+      }
+      if(lane == 0) share = w;
+   }
    __syncthreads();
+   if(share.b0 < 0) return;   // nothing left for this CTA
 
    float2 acc[NS][CH / 2];
 #pragma unroll
@@ -574,8 +719,9 @@ __global__ void __launch_bounds__(THREADS, 1) conv_pipe_kernel(const __grid_cons
       // for the slot's next phase while the first still waits for this one, and take this one's parity for it.
       const int st = warp - CONSUMERS, x = (MX8 ? c0 : c0 / 2) / 4;
       if(st < g.stages) {
-         if(g.quads) fill<TT, HEAD, NS, 4>(&codes_map, &taps_map, p, g, ring, full, empty, flags, entry, rows[st], st, n, worker, workers, longest, mine, b0, c0, x, blocks, lane);
-         else fill<TT, HEAD, NS, 1>(&codes_map, &taps_map, p, g, ring, full, empty, flags, entry, rows[st], st, n, worker, workers, longest, mine, b0, c0, x, blocks, lane);
+         const int mine = b_length<NS>(a, p, share.b0, lane);
+         if(g.quads) fill<TT, HEAD, NS, 4>(&codes_map, &taps_map, p, g, ring, full, empty, flags, entry, rows[st], st, share, mine, c0, x, blocks, lane);
+         else fill<TT, HEAD, NS, 1>(&codes_map, &taps_map, p, g, ring, full, empty, flags, entry, rows[st], st, share, mine, c0, x, blocks, lane);
       }
    } else {
       Path w;
@@ -592,13 +738,14 @@ __global__ void __launch_bounds__(THREADS, 1) conv_pipe_kernel(const __grid_cons
       int st = 0;
       uint32_t phase = 0;
       const uint8_t* at = ring;
-      for(int i = 0; i < n; ++i) {
+      for(int i = 0, n = share.n; i < n; ++i) {
          if(!mbar_wait(full + st, phase, g.status)) break;
          const uint32_t f = flags[st];
          const int count = f & 0xffff;
          if(sums) {
-            if(f <= 0xffff) sum_stage<MX8, TT, HEAD, NS, true>(at, w, count, acc);
-            else sum_stage<MX8, TT, HEAD, NS, false>(at, w, count, acc);
+            if(f <= 0xffff) sum_stage<MX8, TT, HEAD, NS, Sum::ALL>(at, w, count, acc);
+            else if(!(f & NO_HALF)) sum_stage<MX8, TT, HEAD, NS, Sum::FAST>(at, w, count, acc);
+            else sum_stage<MX8, TT, HEAD, NS, Sum::ANY>(at, w, count, acc);
          }
          __syncwarp();
          if(lane == 0) tc::arrive_own(empty + st);
@@ -613,12 +760,13 @@ __global__ void __launch_bounds__(THREADS, 1) conv_pipe_kernel(const __grid_cons
    __syncthreads();   // the ring is done with: every stage that was filled has been waited for
    float* joined = reinterpret_cast<float*>(ring);
    if(warp < CONSUMERS && slot < slots) park<NS>(joined, acc, slot, unit, slots, a.lanes);
-   join<NS>(joined, a, p, a.lanes * CH, slots, THREADS, rank, b0, c0);
+   join<NS>(joined, a, p, a.lanes * CH, slots, THREADS, rank, share.b0, c0, (long long)blockIdx.x * NS);
 }
 
 struct Plan {
-   int ns, lanes, chunks, slots, split, outer, lags, stages;
+   int ns, lanes, chunks, slots, split, pool, lags, stages;
    int row_bytes, tap_bytes, codes_at, scales_at, stage_bytes;
+   size_t partials(int channels) const { return (size_t)pool * ns * channels * sizeof(float); }
 };
 constexpr int SMEM = 200 * 1024;
 
@@ -631,8 +779,9 @@ bool plan(long long lags, bool mx8, int channels, int batch, int tap_size, int s
    p->ns = batch > 2 ? 4 : batch;
    const long long groups = mx::ceil_div(batch, p->ns);
    // A cluster of eight joins short histories in the same launch; long ones
-   // are split over as many CTAs as the card takes at once, and joined by a
-   // second launch.
+   // are dealt to as many CTAs as the card takes at once, and joined by a
+   // second launch (MX4 x 2048, one sequence of 32768 and 15 of 100: an equal
+   // share for each group 194 us, dealt 73).
    const double value = mx8 ? 33.0 / 32 : 17.0 / 32;
    const bool small = (double)lags * channels * (batch * value + tap_size) < 64.0 * (1 << 20);
    // scales that have to be read byte by byte are worth it for long histories only (5 x 5000 x 2112 MX4: 105 us, 65
@@ -641,12 +790,12 @@ bool plan(long long lags, bool mx8, int channels, int batch, int tap_size, int s
    const auto lay = [&](int chunks) {
       p->lanes = (int)mx::ceil_div(mx::ceil_div(units, chunks), grain) * grain;
       p->chunks = (int)mx::ceil_div(units, p->lanes);
-      const int most = small ? MAX_SPLIT : (int)mx::ceil_div(lags, 256);
+      const int most = small ? MAX_SPLIT : groups > MAX_GROUPS ? 1 : (int)mx::ceil_div(lags, 256);
       int w = (int)std::max<long long>(1, std::min<long long>(most, sms / (p->chunks * groups)));
       if(small)
          while(w & (w - 1)) w &= w - 1;   // clusters of 1, 2, 4 or 8
       p->split = small ? w : 1;
-      p->outer = small ? 1 : w;
+      p->pool = small || w == 1 ? 0 : (int)std::min<long long>(most * groups, sms / p->chunks);
       p->row_bytes = p->lanes * (mx8 ? CH : CH / 2);
       p->tap_bytes = tap_size ? p->lanes * CH * tap_size : p->lanes / 2 * 4;
       const int per_lag = p->tap_bytes + p->ns * (p->row_bytes + p->lanes / 2 * 4);
@@ -660,7 +809,7 @@ bool plan(long long lags, bool mx8, int channels, int batch, int tap_size, int s
       p->scales_at = p->codes_at + p->lags * p->ns * p->row_bytes;
       p->stage_bytes = (int)mx::ceil_div(p->lags * per_lag + 128, 1024) * 1024;
       p->stages = std::min(MAX_STAGES, SMEM / p->stage_bytes);
-      return p->chunks * groups * w;   // CTAs
+      return p->pool ? (long long)p->chunks * p->pool : p->chunks * groups * w;   // CTAs
    };
    // chunks of 1024 channels, or of fewer where the card would not be full or the ring not four stages long
    int chunks = (int)mx::ceil_div(units, 64);
@@ -683,7 +832,7 @@ fufft_status launch(const fufft_cache* c, const Args& g, const CUtensorMap& cm, 
    fufft_status s = allow_smem(kern, SMEM + 1024, configured);
    if(s != FUFFT_OK) return s;
    cudaLaunchConfig_t cfg = {};
-   cfg.gridDim = dim3((unsigned)(p.split * p.outer), (unsigned)p.chunks, (unsigned)mx::ceil_div(c->batch, NS));
+   cfg.gridDim = dim3((unsigned)(p.pool ? p.pool : p.split), (unsigned)p.chunks, p.pool ? 1u : (unsigned)mx::ceil_div(c->batch, NS));
    cfg.blockDim = dim3(THREADS);
    cfg.dynamicSmemBytes = smem_of(p);
    cfg.stream = st;
@@ -695,7 +844,10 @@ fufft_status launch(const fufft_cache* c, const Args& g, const CUtensorMap& cm, 
    cfg.numAttrs = 1;
    if((s = check(cudaLaunchKernelEx(&cfg, kern, cm, tm, Pages(c), g))) != FUFFT_OK) return s;
    count_launch();
-   return FUFFT_OK;
+   if(!p.pool) return FUFFT_OK;
+   join_dealt_kernel<NS><<<(unsigned)mx::ceil_div((long long)c->batch * c->channels, 256), 256, 0, st>>>(g.a, c->batch, p.lags, p.pool);
+   count_launch();
+   return check(cudaGetLastError());
 }
 template<bool MX8, class TT, bool HEAD>
 fufft_status launch(const fufft_cache* c, const Args& g, const CUtensorMap& cm, const CUtensorMap& tm, const Plan& p, cudaStream_t st)
@@ -829,11 +981,11 @@ size_t fufft_cache_conv_workspace(const fufft_cache* c, int64_t n_taps)
    if(cudaGetDevice(&dev) != cudaSuccess) return 0;
    const long long lags = cache::lags_of(c, n_taps);
    const int sms = sm_count(dev);
-   int outer = cache::plan(lags, c->channels, c->batch, sms).outer;
+   size_t need = cache::partials(cache::plan(lags, c->channels, c->batch, sms).outer, c);
    cache::pipe::Plan p;   // whichever way the taps will lie
    for(int tap_size : {0, 2, 4})
-      if(cache::pipe::plan(lags, c->kind == FUFFT_CACHE_MX8, c->channels, c->batch, tap_size, sms, &p)) outer = std::max(outer, p.outer);
-   return cache::partials(outer, c);
+      if(cache::pipe::plan(lags, c->kind == FUFFT_CACHE_MX8, c->channels, c->batch, tap_size, sms, &p)) need = std::max(need, p.partials(c->channels));
+   return need;
 }
 
 fufft_status fufft_cache_conv(const fufft_cache* c, const int32_t* lengths, const void* taps, fufft_dtype taps_dtype,
@@ -878,7 +1030,7 @@ fufft_status fufft_cache_conv(const fufft_cache* c, const int32_t* lengths, cons
    const bool shared = a.group % mx::BLOCK == 0;
    if((shared || (a.group == 1 && a.vec_taps)) &&
       c->pages > 0 && cache::pipe::plan(lags, mx8, c->channels, c->batch, shared ? 0 : tap_size, sm_count(dev), &pp)) {
-      const size_t need = cache::partials(pp.outer, c);
+      const size_t need = pp.partials(c->channels);
       if(workspace_bytes < need || (need && !workspace)) return FUFFT_ERR_INVALID_ARG;
       DeviceCtx ctx;
       if((s = device_ctx(&ctx)) != FUFFT_OK) return s;
@@ -886,15 +1038,14 @@ fufft_status fufft_cache_conv(const fufft_cache* c, const int32_t* lengths, cons
       a.lanes = pp.lanes;
       a.slots = pp.slots;
       a.split = pp.split;
-      a.outer = pp.outer;
       CUtensorMap tm{}, cm;
       if((s = cache::pipe::codes_tmap(&cm, c, pp)) != FUFFT_OK) return s;
       if(!shared && (s = cache::pipe::taps_tmap(&tm, a, tap_size, pp)) != FUFFT_OK) return s;
-      const cache::pipe::Args g{a, ctx.status, pp.lags, pp.stages, pp.stage_bytes, pp.codes_at, pp.scales_at, pp.row_bytes, pp.tap_bytes,
+      const cache::pipe::Args g{a, ctx.status, pp.lags, pp.stages, pp.stage_bytes, pp.codes_at, pp.scales_at, pp.row_bytes, pp.tap_bytes, pp.pool,
                                 c->channels % 128 == 0 && pp.lanes % 8 == 0};
       if(mx8) s = tap_size == 4 ? cache::pipe::launch<true, float>(c, g, shared, cm, tm, pp, st) : cache::pipe::launch<true, __nv_bfloat16>(c, g, shared, cm, tm, pp, st);
       else s = tap_size == 4 ? cache::pipe::launch<false, float>(c, g, shared, cm, tm, pp, st) : cache::pipe::launch<false, __nv_bfloat16>(c, g, shared, cm, tm, pp, st);
-      return s != FUFFT_OK || pp.outer == 1 ? s : cache::join_clusters(a, c->batch, st);
+      return s;
    }
    const cache::Plan p = cache::plan(lags, c->channels, c->batch, sm_count(dev));
    const size_t need = cache::partials(p.outer, c);

@@ -227,6 +227,33 @@ def test_conv_long(ops, kind, heads):
 
 
 @gpu
+@pytest.mark.parametrize("spread", ["one", "none", "equal", "falling", "any"])
+def test_conv_long_unequal(ops, spread):
+    """ten groups of sequences whose lengths decide how many CTAs each of them gets"""
+    g = torch.Generator(device="cuda").manual_seed(41)
+    batch, n, channels, page = 37, 8192, 512, 64
+    lengths = {"one": [0] * 30 + [8192] + [0] * 6, "none": [0] * 37, "equal": [8192] * 37,
+               "falling": [8192 - 220 * b for b in range(37)],
+               "any": torch.randint(0, 8193, (37,), generator=torch.Generator().manual_seed(3)).tolist()}[spread]
+    per = n // page
+    table = torch.randperm(batch * per, device="cuda", generator=g).view(batch, per).int()
+    cache = ops.seq_cache(batch * per, page, channels, table, "mx4")
+    cache.codes.random_(0, 256, generator=g)
+    cache.scales.random_(120, 131, generator=g)
+    lens = torch.tensor(lengths, dtype=torch.int32)
+    cu, zero = _cu(lengths).cuda(), torch.zeros(batch, dtype=torch.int32, device="cuda")
+    stored = ops.cache_read(cache, cu, zero, sum(lengths), torch.float32).split(lengths)
+    for taps_dtype, heads in ((torch.float32, 512), (torch.bfloat16, 16)):
+        taps = torch.randn(n, heads, device="cuda", generator=g).to(taps_dtype)
+        got = ops.cache_conv(cache, lens.cuda(), taps, dtype=torch.float32).double()
+        for b, v in enumerate(stored):
+            t = v.flip(0).double() * taps[:len(v)].double().repeat_interleave(channels // heads, 1)
+            tol = ref.sum_tolerance(t.sum(0), t.abs().sum(0), len(v), torch.float32)
+            assert bool(((got[b] - t.sum(0)).abs() <= tol).all())
+        assert torch.equal(ops.cache_conv(cache, lens.cuda(), taps, dtype=torch.float32).double(), got)
+
+
+@gpu
 def test_conv_strides_and_repeats(ops):
     """taps, gate and result as parts of wider rows, unaligned among them; the same bits on every call"""
     m = Model(ops, 3, 900, 96, 16, "mx4", seed=8)
