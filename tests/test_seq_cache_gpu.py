@@ -346,6 +346,35 @@ def test_empty(ops):
 
 
 @gpu
+@pytest.mark.parametrize("channels", [96, 2048])
+def test_no_pages(ops, channels):
+    """lengths and a page table, but no page at all: nothing is read, and the outputs are zeros"""
+    table = torch.zeros(2, 100, dtype=torch.int32, device="cuda")
+    none = ops.seq_cache(0, 16, channels, table)
+    lengths = torch.tensor([1600, 3], dtype=torch.int32, device="cuda")
+    for heads in (channels, channels // 32, 3 if channels == 96 else 256):
+        out = ops.cache_conv(none, lengths, torch.full((700, heads), float("inf"), device="cuda"), dtype=torch.float32)
+        assert bool((out == 0).all())
+
+
+@gpu
+def test_conv_non_finite_taps(ops):
+    """a tap that is infinite or NaN meets only rows that are there, in both kernels"""
+    for channels, batch in ((96, 3), (1024, 4)):
+        m = Model(ops, batch, 900, channels, 16, "mx4", seed=13)
+        lengths = [900, 70, 450, 0][:batch]
+        m.append(lengths, torch.float32)
+        taps = torch.randn(900, channels, generator=m.g)
+        taps[500:], taps[890:] = float("inf"), float("nan")
+        got = ops.cache_conv(m.cache, m.lengths.cuda(), taps.cuda(), dtype=torch.float32).cpu()
+        assert not bool(got[0].isfinite().any())
+        finite = taps.clone()
+        finite[500:] = 0.0
+        want, tol = _step(m, finite, None, torch.float32)
+        assert bool(((got[1:].double() - want[1:]).abs() <= tol[1:]).all())
+
+
+@gpu
 def test_refusals(ops):
     m = Model(ops, 2, 32, 64, 16, "mx4")
     c, cu, at = m.cache, _cu([1, 1]).cuda(), torch.zeros(2, dtype=torch.int32, device="cuda")
