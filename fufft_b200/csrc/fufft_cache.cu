@@ -149,7 +149,8 @@ __global__ void __launch_bounds__(THREADS) read_kernel(T* __restrict__ out, long
 // positions out, 16 bytes each.  The tile is skewed by 8 words per 16
 // channels: the lanes of a warp, 8 positions x 4 groups of channels, store
 // into 32 banks.  Bound by writing the rows, padding and all (8 x 4096 x 16384
-// fp32 from 8192 tokens MX4: 430 us, floor 349).
+// fp32 from 8192 tokens MX4: 433 us, floor 349; MX8 449, floor 370, and 489 with
+// loads under conditions).
 constexpr int RN = 128, RC = 64, RPITCH = RN + 4;
 template<class T, bool MX8>
 __global__ void __launch_bounds__(THREADS) read_channels_kernel(T* __restrict__ out, Pages p,
@@ -165,7 +166,7 @@ __global__ void __launch_bounds__(THREADS) read_channels_kernel(T* __restrict__ 
    const int b = (int)(rest / tiles_c), c0 = (int)(rest % tiles_c) * RC;
    const long long i0 = (long long)(id % tiles_n) * RN;
    const long long count = min((long long)counts[b], n);
-   const bool any = i0 < count;
+   const bool any = i0 < count && p.pages > 0;
    if(any) {
       if(threadIdx.x < RN) {
          const long long i = i0 + threadIdx.x;
@@ -173,17 +174,16 @@ __global__ void __launch_bounds__(THREADS) read_channels_kernel(T* __restrict__ 
       }
       __syncthreads();
       uint32_t q[2][E::WORDS], s[2];
+      bool there[2];
 #pragma unroll
       for(int k = 0; k < 2; ++k) {
          const int r = k * 64 + (threadIdx.x >> 2), c = c0 + (threadIdx.x & 3) * mx::HALF;
-         const int row = c < channels ? rows[r] : -1;
-#pragma unroll
-         for(int i = 0; i < E::WORDS; ++i) q[k][i] = 0;
-         s[k] = 0;
-         if(row >= 0) {
-            mx::load_codes<E::WORDS>(p.codes + ((long long)row * (channels / mx::HALF) + c / mx::HALF) * (4 * E::WORDS), q[k]);
-            s[k] = __ldg(p.scales + (long long)row * (channels / mx::BLOCK) + c / mx::BLOCK);
-         }
+         there[k] = c < channels && rows[r] >= 0;
+         // loads without a condition, the first row's where there is none: what a branch may or may not have loaded
+         // is waited for where the branch ends
+         const long long row = there[k] ? rows[r] : 0, at = there[k] ? c : 0;
+         mx::load_codes<E::WORDS>(p.codes + (row * (channels / mx::HALF) + at / mx::HALF) * (4 * E::WORDS), q[k]);
+         s[k] = __ldg(p.scales + row * (channels / mx::BLOCK) + at / mx::BLOCK);
       }
 #pragma unroll
       for(int k = 0; k < 2; ++k) {
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(THREADS) read_channels_kernel(T* __restrict__ 
          float v[mx::HALF];
          mx::decode<MX8>(q[k], mx::scale_value(s[k]), v);
 #pragma unroll
-         for(int i = 0; i < mx::HALF; ++i) tile[(g * mx::HALF + i) * RPITCH + g * 8 + r] = v[i];
+         for(int i = 0; i < mx::HALF; ++i) tile[(g * mx::HALF + i) * RPITCH + g * 8 + r] = there[k] ? v[i] : 0.0f;
       }
       __syncthreads();
    }

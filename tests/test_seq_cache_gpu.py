@@ -355,6 +355,7 @@ def test_no_pages(ops, channels):
     for heads in (channels, channels // 32, 3 if channels == 96 else 256):
         out = ops.cache_conv(none, lengths, torch.full((700, heads), float("inf"), device="cuda"), dtype=torch.float32)
         assert bool((out == 0).all())
+    assert bool((ops.cache_read_channels(none, lengths - lengths, lengths, 300) == 0).all())
 
 
 @gpu
