@@ -3,6 +3,7 @@
 //   y[b][c] = gate[b][c] * sum_{j < min(len_b, L)} taps[j][head(c)] * x[b][len_b - 1 - j][c]
 // with head(c) = c / (channels / heads).
 #include <algorithm>
+#include <type_traits>
 
 #include "fufft_cache.cuh"
 #include "fufft_tc.cuh"
@@ -74,6 +75,16 @@ __device__ __forceinline__ float2 ffma2(float2 a, float2 b, float2 c)
    asm("{\n\t.reg .b64 ra, rb, rc, rr;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmov.b64 rc, {%6, %7};\n\t"
        "fma.rn.f32x2 rr, ra, rb, rc;\n\tmov.b64 {%0, %1}, rr;\n\t}"
        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+   return r;
+}
+
+// x times scale, halves widened: exact
+__device__ __forceinline__ float2 widen_scaled(uint32_t x, uint32_t scale)
+{
+   float2 r;
+   asm("{\n\t.reg .b16 a, b, c, d;\n\tmov.b32 {a, b}, %2;\n\tmov.b32 {c, d}, %3;\n\t"
+       "fma.rn.f32.f16 %0, a, c, %4;\n\tfma.rn.f32.f16 %1, b, c, %4;\n\t}"
+       : "=f"(r.x), "=f"(r.y) : "r"(x), "r"(scale), "f"(0.0f));
    return r;
 }
 
@@ -164,8 +175,12 @@ __device__ __forceinline__ void join(float* joined, const ConvStep& a, const Pag
 
 // A CTA: a.lanes x 16 channels of NB sequences, a.slots lags at a time; the
 // same taps serve the NB sequences, which stand at different positions of
-// their pages but at the same lag.  Per stored value: half a conversion, one
-// widening, half a product of scale and tap, half a sum (packed pairs).
+// their pages but at the same lag.  A value is scaled before it meets the tap:
+// a stored value is a number of 32 bits, exactly, where a scale of 2^124 times
+// a tap need not be.  One exact fma widens and scales it where the scale is a
+// half-precision number, two operations where a scale of the thread's batch is
+// not (5 x 5000 x 2112 MX4, 22 heads: 12.7 us, 14.8 if all took two); half a
+// packed fma adds it times its tap.
 // CTAs of a cluster take tiles of lags in turn and join through distributed
 // shared memory, in rank order.
 template<bool MX8, class TT, Taps MODE, int NB>
@@ -212,7 +227,7 @@ __global__ void __launch_bounds__(THREADS, 2) conv_step_kernel(Pages p, ConvStep
          uint32_t there = 0;   // which of them are
          TapRow<TT, MODE> h[U];
          // loads without a condition, the first row's where there is none: what a branch may or may not have loaded
-         // is waited for where the branch ends (5 x 5000 x 2112 MX4, 22 heads: 14.6 us, under conditions 18.0)
+         // is waited for where the branch ends
 #pragma unroll
          for(int u = 0; u < U; ++u) {
             const int ju = min(j + u * a.slots, count - 1);
@@ -225,18 +240,33 @@ __global__ void __launch_bounds__(THREADS, 2) conv_step_kernel(Pages p, ConvStep
                sc[u][s] = __ldg(scales + (long long)max(row, 0) * row_scales);
             }
          }
+         uint32_t widest = 0;   // below 30: all scales are 2^-14 .. 2^15, normal halves
 #pragma unroll
          for(int u = 0; u < U; ++u)
 #pragma unroll
-            for(int s = 0; s < NB; ++s) {
-               if(!(there >> (u * NB + s) & 1)) continue;
-               const float scale = mx::scale_value(sc[u][s]);
-               uint32_t v[CH / 2];
-               q[u][s].halves(v);
+            for(int s = 0; s < NB; ++s) widest = max(widest, sc[u][s] - 113u);
+         const auto sum = [&](auto halves) {
 #pragma unroll
-               for(int i = 0; i < CH / 2; ++i)
-                  acc[s][i] = ffma2(mx::half2_f(v[i]), fmul2(h[u].pair(i), make_float2(scale, scale)), acc[s][i]);
-            }
+            for(int u = 0; u < U; ++u)
+#pragma unroll
+               for(int s = 0; s < NB; ++s) {
+                  if(!(there >> (u * NB + s) & 1)) continue;
+                  uint32_t v[CH / 2];
+                  q[u][s].halves(v);
+                  if constexpr(halves.value) {
+                     const uint32_t scale = (sc[u][s] - 112u) << 10;
+#pragma unroll
+                     for(int i = 0; i < CH / 2; ++i) acc[s][i] = ffma2(widen_scaled(v[i], scale), h[u].pair(i), acc[s][i]);
+                  } else {
+                     const float scale = mx::scale_value(sc[u][s]);
+#pragma unroll
+                     for(int i = 0; i < CH / 2; ++i)
+                        acc[s][i] = ffma2(fmul2(mx::half2_f(v[i]), make_float2(scale, scale)), h[u].pair(i), acc[s][i]);
+                  }
+               }
+         };
+         if(widest < 30u) sum(std::true_type());
+         else sum(std::false_type());
       }
    }
 
@@ -388,16 +418,6 @@ __device__ __forceinline__ void gather4(const CUtensorMap* tm, void* dst, int x,
    asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
                 :: "r"(smem_u32(dst)), "l"(tm), "r"(x), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w), "r"(smem_u32(bar)) : "memory");
 }
-// x times scale, halves widened: exact
-__device__ __forceinline__ float2 widen_scaled(uint32_t x, uint32_t scale)
-{
-   float2 r;
-   asm("{\n\t.reg .b16 a, b, c, d;\n\tmov.b32 {a, b}, %2;\n\tmov.b32 {c, d}, %3;\n\t"
-       "fma.rn.f32.f16 %0, a, c, %4;\n\tfma.rn.f32.f16 %1, b, c, %4;\n\t}"
-       : "=f"(r.x), "=f"(r.y) : "r"(x), "r"(scale), "f"(0.0f));
-   return r;
-}
-
 // A scale as a stage holds it: the half-precision number in the low half, its byte in bits 16 .. 23.
 constexpr uint32_t NO_HALF = 1u << 31, NO_ROW = 1u << 30;
 __device__ __forceinline__ uint32_t scale_entry(uint32_t s)
