@@ -416,15 +416,14 @@ def pipeline_v16_bfp(aq, a_scale, bq, b_scale, n):
 # These operators run at a few microseconds, the time of their own Python: one
 # allocation for the two buffers of a matrix, no check made twice.
 _DTYPES = {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}
-_raw_stream, _device_index = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
 def _queue(t: torch.Tensor) -> int:
     """the current stream of the current device, as _stream, without making a stream object; t has to be there"""
-    device = _device_index()
+    device = torch._C._cuda_getDevice()   # looked up here: a torch without CUDA has no such name, and still imports this
     if t.get_device() != device:
         raise ValueError(f"the tensors are on cuda:{t.get_device()}, the current device is cuda:{device}")
-    return _raw_stream(device)
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def _dtype(t: torch.dtype) -> int:
