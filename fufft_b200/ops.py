@@ -418,11 +418,13 @@ def pipeline_v16_bfp(aq, a_scale, bq, b_scale, n):
 _DTYPES = {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}
 
 
-def _queue(t: torch.Tensor) -> int:
-    """the current stream of the current device, as _stream, without making a stream object; t has to be there"""
+def _queue(*operands) -> int:
+    """the current stream of the current device, as _stream, without making a stream object; every operand of the call
+    (tensors, Mx4, SeqCache, None) has to be there, since only its address goes on"""
     device = torch._C._cuda_getDevice()   # looked up here: a torch without CUDA has no such name, and still imports this
-    if t.get_device() != device:
-        raise ValueError(f"the tensors are on cuda:{t.get_device()}, the current device is cuda:{device}")
+    for t in operands:
+        if t is not None and t.get_device() != device:
+            raise ValueError(f"an operand is on cuda:{t.get_device()}, the current device is cuda:{device}")
     return torch._C._cuda_getCurrentRawStream(device)
 
 
@@ -466,7 +468,7 @@ class Mx4:
     codes uint8 [rows, ceil(cols / 256) * 128] and the tiled E8M0 scales uint8
     [ceil(rows / 128), ceil(cols / 256) * 2, 32, 4, 4] (layout in
     include/fufft_b200.h, fufft_mx4_*)"""
-    __slots__ = ("_codes", "_scales", "_buffer", "rows", "cols", "at")
+    __slots__ = ("_codes", "_scales", "_buffer", "_device", "rows", "cols", "at")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, cols: int):
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
@@ -476,6 +478,13 @@ class Mx4:
             raise ValueError(f"codes or scales do not fit a {rows} x {cols} matrix")
         self._codes, self._scales, self._buffer, self.rows, self.cols = codes, scales, codes, rows, cols
         self.at = _ptr(codes), _ptr(scales)
+        self._device = codes.get_device()
+        if scales.get_device() != self._device:
+            raise ValueError(f"codes are on cuda:{self._device}, scales on cuda:{scales.get_device()}")
+
+    def get_device(self) -> int:
+        """index of the device, as a tensor's"""
+        return self._device
 
     @property
     def codes(self) -> torch.Tensor:
@@ -504,7 +513,7 @@ def _mx4_new(like: torch.Tensor, rows: int, cols: int) -> Mx4:
     codes = rows * tiles * 64          # a multiple of 128
     q._buffer = like.new_empty(codes + -(-rows // 128) * tiles * 512, dtype=torch.uint8)
     q._codes = q._scales = None
-    q.rows, q.cols = rows, cols
+    q._device, q.rows, q.cols = q._buffer.get_device(), rows, cols
     at = q._buffer.data_ptr()
     q.at = at, at + codes
     return q
@@ -556,7 +565,7 @@ def mx4_dequantize(q: Mx4, dtype: torch.dtype = torch.float32, out: torch.Tensor
     """the values that q stands for"""
     code = _dtype(dtype)
     out, pitch = _result(out, q._buffer, q.rows, q.cols, dtype)
-    rc = lib().fufft_mx4_dequantize(*q.at, q.rows, q.cols, out.data_ptr(), code, pitch, _queue(out))
+    rc = lib().fufft_mx4_dequantize(*q.at, q.rows, q.cols, out.data_ptr(), code, pitch, _queue(q, out))
     if rc:
         check(rc, "fufft_mx4_dequantize")
     return out
@@ -577,7 +586,7 @@ def mx4_matmul(a: Mx4, b: Mx4, dtype: torch.dtype = torch.bfloat16, bias: torch.
     code = _dtype(dtype)
     out, pitch = _result(out, a._buffer, a.rows, b.rows, dtype)
     rc = lib().fufft_mx4_matmul(*a.at, *b.at, _bias(bias, b.rows), out.data_ptr(), code, a.rows, b.rows, a.cols, pitch,
-                                _queue(out))
+                                _queue(a, b, bias, out))
     if rc:
         check(rc, "fufft_mx4_matmul")
     return out
@@ -597,7 +606,7 @@ def mx4_linear(x: torch.Tensor, w: Mx4, bias: torch.Tensor | None = None,
     out = flat.new_empty((m, w.rows), dtype=dtype)
     q = None if m <= MX4_DIRECT_ROWS else _mx4_new(flat, m, k)   # few rows are quantised inside the product
     rc = lib().fufft_mx4_linear(flat.data_ptr(), codes, m, k, pitch, *(q.at if q else (None, None)), *w.at, w.rows,
-                                _bias(bias, w.rows), out.data_ptr(), out_code, w.rows, _queue(out))
+                                _bias(bias, w.rows), out.data_ptr(), out_code, w.rows, _queue(flat, w, bias))
     if rc:
         check(rc, "fufft_mx4_linear")
     return out if x.dim() == 2 else out.view(*x.shape[:-1], w.rows)
@@ -625,7 +634,7 @@ class SeqCache:
       codes       uint8 [pages, page_size, channels / 2 (mx4) or channels (mx8)]
       scales      uint8 [pages, page_size, channels / 32]
       page_table  int32 [batch, max_pages], -1 where there is no page"""
-    __slots__ = ("codes", "scales", "page_table", "kind", "channels", "batch", "desc", "at")
+    __slots__ = ("codes", "scales", "page_table", "kind", "channels", "batch", "desc", "at", "_device")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, page_table: torch.Tensor, kind: str):
         code = _KINDS.get(kind)
@@ -644,6 +653,14 @@ class SeqCache:
         self.desc = CacheDesc(_ptr(codes), _ptr(scales), page_table.data_ptr(), stride, code, channels, page_size, pages,
                               max_pages, self.batch)
         self.at = ct.addressof(self.desc)
+        self._device = codes.get_device()
+        if scales.get_device() != self._device or page_table.get_device() != self._device:
+            raise ValueError(f"codes are on cuda:{self._device}, scales on cuda:{scales.get_device()}, "
+                             f"page_table on cuda:{page_table.get_device()}")
+
+    def get_device(self) -> int:
+        """index of the device, as a tensor's"""
+        return self._device
 
 
 def seq_cache(pages: int, page_size: int, channels: int, page_table: torch.Tensor, kind: str = "mx8") -> SeqCache:
@@ -662,7 +679,7 @@ def cache_append(cache: SeqCache, x: torch.Tensor, cu: torch.Tensor, starts: tor
     if channels != cache.channels:
         raise ValueError(f"x must have {cache.channels} channels")
     rc = lib().fufft_cache_append(cache.at, x.data_ptr(), _dtype(x.dtype), pitch, _i32(cu, cache.batch + 1, "cu"),
-                                  _i32(starts, cache.batch, "starts"), tokens, _queue(x))
+                                  _i32(starts, cache.batch, "starts"), tokens, _queue(cache, x, cu, starts))
     if rc:
         check(rc, "fufft_cache_append")
 
@@ -675,7 +692,7 @@ def cache_read(cache: SeqCache, cu: torch.Tensor, starts: torch.Tensor, tokens: 
     if cache.batch == 0:
         out.zero_()
     rc = lib().fufft_cache_read(cache.at, out.data_ptr(), code, pitch, _i32(cu, cache.batch + 1, "cu"),
-                                _i32(starts, cache.batch, "starts"), tokens, _queue(out))
+                                _i32(starts, cache.batch, "starts"), tokens, _queue(cache, cu, starts, out))
     if rc:
         check(rc, "fufft_cache_read")
     return out
@@ -689,7 +706,7 @@ def cache_read_channels(cache: SeqCache, starts: torch.Tensor, counts: torch.Ten
     code = _dtype(dtype)
     out = cache.codes.new_empty((cache.batch, cache.channels, n), dtype=dtype)
     rc = lib().fufft_cache_read_channels(cache.at, out.data_ptr(), code, n, _i32(starts, cache.batch, "starts"),
-                                         _i32(counts, cache.batch, "counts"), _queue(out))
+                                         _i32(counts, cache.batch, "counts"), _queue(cache, starts, counts))
     if rc:
         check(rc, "fufft_cache_read_channels")
     return out
@@ -718,7 +735,8 @@ def cache_conv(cache: SeqCache, lengths: torch.Tensor, taps: torch.Tensor, gate:
             workspace = out.new_empty(need, dtype=torch.uint8)
     rc = lib().fufft_cache_conv(cache.at, _i32(lengths, cache.batch, "lengths"), taps.data_ptr(), _DTYPES[taps.dtype], n,
                                 heads, taps_pitch, gate_at, gate_pitch, out.data_ptr(), code, pitch, _ptr(workspace),
-                                0 if workspace is None else workspace.numel(), _queue(out))
+                                0 if workspace is None else workspace.numel(),
+                                _queue(cache, lengths, taps, gate, out, workspace))
     if rc:
         check(rc, "fufft_cache_conv")
     return out
