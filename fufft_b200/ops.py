@@ -612,16 +612,19 @@ def mx4_linear(x: torch.Tensor, w: Mx4, bias: torch.Tensor | None = None,
     return out if x.dim() == 2 else out.view(*x.shape[:-1], w.rows)
 
 
-def mx4_linear_grad(gy: torch.Tensor, xt: Mx4, wt: Mx4,
-                    dtype: torch.dtype | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+def mx4_linear_grad(gy: torch.Tensor, xt: Mx4, wt: Mx4, dtype: torch.dtype | None = None,
+                    w_dtype: torch.dtype | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """gradients of y = x w^T [m, n] with every operand in 4 bits, the
     quantiser passed straight through: gx [m, k] = Q(gy) Q(w^T)^T and
     gw [n, k] = Q(gy^T) Q(x^T)^T, from xt = mx4_quantize(x, transpose=True)
-    [k, m] and wt = mx4_quantize(w, transpose=True) [k, n]"""
+    [k, m] and wt = mx4_quantize(w, transpose=True) [k, n].  gx in `dtype`
+    (gy's unless given), gw in `w_dtype` (as gx unless given), each rounded
+    once from its float32 sums"""
     if gy.dim() != 2 or xt.cols != gy.shape[0] or wt.cols != gy.shape[1] or xt.rows != wt.rows:
         raise ValueError(f"gy {tuple(gy.shape)} does not fit xt {xt.shape} and wt {wt.shape}")
     gq, gt = mx4_quantize_both(gy)
-    return mx4_matmul(gq, wt, dtype or gy.dtype), mx4_matmul(gt, xt, dtype or gy.dtype)
+    dtype = dtype or gy.dtype
+    return mx4_matmul(gq, wt, dtype), mx4_matmul(gt, xt, w_dtype or dtype)
 
 
 # ---- quantised sequence cache -----------------------------------------------------------

@@ -12,7 +12,7 @@ and, for the layers around a long convolution,
   torch.ops.fufft.mx4_quantize(x, transpose) -> (codes, scales)
   torch.ops.fufft.mx4_linear(x, w_codes, w_scales, n, bias) -> Tensor
   torch.ops.fufft.mx4_train(x, w) -> (y, xt codes, xt scales, wt codes, wt scales)
-  torch.ops.fufft.mx4_train_grad(gy, xt codes, xt scales, wt codes, wt scales) -> (gx, gw)
+  torch.ops.fufft.mx4_train_grad(gy, xt codes, xt scales, wt codes, wt scales, w_dtype) -> (gx, gw)
   torch.ops.fufft.cache_append(x, codes, scales, page_table, kind, cu, starts) -> ()
   torch.ops.fufft.cache_read(codes, scales, page_table, kind, cu, starts, tokens, dtype) -> Tensor
   torch.ops.fufft.cache_read_channels(codes, scales, page_table, kind, starts, counts, n) -> Tensor
@@ -130,15 +130,16 @@ def _(x, w):
 
 @torch.library.custom_op(f"{_NS}::mx4_train_grad", mutates_args=())
 def mx4_train_grad(gy: torch.Tensor, xt_codes: torch.Tensor, xt_scales: torch.Tensor, wt_codes: torch.Tensor,
-                   wt_scales: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+                   wt_scales: torch.Tensor, w_dtype: torch.dtype | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     k = wt_codes.shape[0]
-    return ops.mx4_linear_grad(gy, ops.Mx4(xt_codes, xt_scales, k, gy.shape[0]), ops.Mx4(wt_codes, wt_scales, k, gy.shape[1]))
+    return ops.mx4_linear_grad(gy, ops.Mx4(xt_codes, xt_scales, k, gy.shape[0]), ops.Mx4(wt_codes, wt_scales, k, gy.shape[1]),
+                               w_dtype=w_dtype)
 
 
 @mx4_train_grad.register_fake
-def _(gy, xt_codes, xt_scales, wt_codes, wt_scales):
+def _(gy, xt_codes, xt_scales, wt_codes, wt_scales, w_dtype=None):
     k = wt_codes.shape[0]
-    return gy.new_empty((gy.shape[0], k)), gy.new_empty((gy.shape[1], k))
+    return gy.new_empty((gy.shape[0], k)), gy.new_empty((gy.shape[1], k), dtype=w_dtype or gy.dtype)
 
 
 def _train_context(ctx, inputs, output):
@@ -147,8 +148,7 @@ def _train_context(ctx, inputs, output):
 
 
 def _train_backward(ctx, gy, *_):
-    gx, gw = torch.ops.fufft.mx4_train_grad(gy.contiguous(), *ctx.saved_tensors)
-    return gx, gw.to(ctx.w_dtype)
+    return torch.ops.fufft.mx4_train_grad(gy.contiguous(), *ctx.saved_tensors, ctx.w_dtype)
 
 
 mx4_train.register_autograd(_train_backward, setup_context=_train_context)
