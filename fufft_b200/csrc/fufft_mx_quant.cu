@@ -87,6 +87,23 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict_
       else if(mine == HALF) h[u].load(at + u * SPAN + lane * HALF);
       else h[u].load_some(at + u * SPAN + lane * HALF, mine);
    }
+   // The last tile's rows that are not there have zeros for scales: dealt to those that are, eight lanes a tile.  Rows
+   // 32 apart are neighbours in a tile.
+   const unsigned tile_rows = min(rows - row / TILE_ROWS * TILE_ROWS, (unsigned)TILE_ROWS);
+   if(tile_rows < TILE_ROWS)
+      for(int u = 0; u < U; ++u) {
+         const long long col = c0 + u * SPAN + lane * HALF;
+         if(col >= pitch * 2) break;
+         uint8_t* words = scales + ((long long)(row / TILE_ROWS) * (pitch / 64) + col / 128) * TILE_BYTES;
+         const unsigned in = row % TILE_ROWS, step = min(tile_rows, 32u);
+         for(unsigned r = in % 32 + step * (lane & 7); in < 32 && r < 32; r += step * 8) {
+            uint32_t* line = reinterpret_cast<uint32_t*>(words + r * 16);
+            if(r >= tile_rows) *reinterpret_cast<uint4*>(line) = make_uint4(0, 0, 0, 0);
+            else
+               for(int k = 1; k < 4; ++k)
+                  if(r + 32 * k >= tile_rows) line[k] = 0u;
+         }
+      }
 #pragma unroll
    for(int u = 0; u < U; ++u) {
       uint32_t c[2];
@@ -141,6 +158,13 @@ __device__ __forceinline__ uint4 encode_block(uint32_t s, const float* v)
 {
    const uint4 q = make_uint4(e2m1_encode8(v), e2m1_encode8(v + 8), e2m1_encode8(v + 16), e2m1_encode8(v + 24));
    return s == 255u ? make_uint4(0, 0, 0, 0) : q;
+}
+
+// a tile's scales of rows that are not there, where some are and some are not
+__device__ __forceinline__ void clear_words(uint8_t* words, long long there)
+{
+   if(there <= 0 || there >= TILE_ROWS) return;
+   for(int r = (int)there + threadIdx.x; r < TILE_ROWS; r += blockDim.x) *reinterpret_cast<uint32_t*>(words + tile_word(r)) = 0u;
 }
 
 template<class T, bool ROWS>
@@ -206,6 +230,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) quantize_tile_ker
          }
       }
    }
+   if constexpr(ROWS) clear_words(scales + (r0 / TILE_ROWS * ct + c0 / QT) * TILE_BYTES, rows - r0);
    __syncthreads();
    const int b = lane & 3;
    uint8_t* scale_tile = scales_t + (c0 / TILE_ROWS * mx4_scale_tiles(rows) + r0 / QT) * TILE_BYTES;
@@ -255,6 +280,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) quantize_tile_ker
          }
       }
    }
+   clear_words(scale_tile, cols - c0);
 }
 
 template<class T, int U>

@@ -405,7 +405,8 @@ fufft_status fufft_conv_large_bfp_noalloc(const int16_t* aq, const float* a_scal
  *           255 = NaN).  Stored in tiles of 128 rows x 4 blocks of 512 bytes,
  *           [ceil(rows / 128)][pitch / 64][32][4][4] = [row tile][block tile]
  *           [row % 32][row / 32 % 4][block % 4]: what the tensor cores take.
- *           Bytes of rows beyond `rows` are never used.
+ *           Bytes of rows beyond `rows` are zeros as quantize writes them,
+ *           and never used.
  *   s - 127 = max(-127, floor(log2(max|x|)) - 2); elements are x / scale
  *   rounded to nearest even, saturating at 6.  An infinity or a NaN makes its
  *   whole block NaN.
