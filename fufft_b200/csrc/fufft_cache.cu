@@ -322,8 +322,8 @@ fufft_status fufft_cache_read(const fufft_cache* c, void* out, fufft_dtype dtype
    if(s != FUFFT_OK) return s;
    if(bad_dtype(dtype)) return FUFFT_ERR_INVALID_ARG;
    if(tokens < 0 || tokens > cache::MAX_TOKENS) return FUFFT_ERR_INVALID_SIZE;
-   if(tokens == 0 || c->batch == 0) return FUFFT_OK;
-   if(!out || !cu || !starts || (row_stride < c->channels && tokens > 1)) return FUFFT_ERR_INVALID_ARG;
+   if(tokens == 0) return FUFFT_OK;
+   if(!out || !cu || (!starts && c->batch) || (row_stride < c->channels && tokens > 1)) return FUFFT_ERR_INVALID_ARG;
    if(!aligned(out, dtype_align(dtype)) || !aligned(cu, 4) || !aligned(starts, 4)) return FUFFT_ERR_MISALIGNED;
    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
    switch(dtype) {

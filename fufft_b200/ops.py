@@ -692,8 +692,6 @@ def cache_read(cache: SeqCache, cu: torch.Tensor, starts: torch.Tensor, tokens: 
     """stored values [tokens, channels] of the ragged run (cu, starts), as in cache_append"""
     code = _dtype(dtype)
     out, pitch = _result(out, cache.codes, tokens, cache.channels, dtype)
-    if cache.batch == 0:
-        out.zero_()
     rc = lib().fufft_cache_read(cache.at, out.data_ptr(), code, pitch, _i32(cu, cache.batch + 1, "cu"),
                                 _i32(starts, cache.batch, "starts"), tokens, _queue(cache, cu, starts, out))
     if rc:
