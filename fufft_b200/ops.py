@@ -595,7 +595,7 @@ def mx4_matmul(a: Mx4, b: Mx4, dtype: torch.dtype = torch.bfloat16, bias: torch.
 def mx4_linear(x: torch.Tensor, w: Mx4, bias: torch.Tensor | None = None,
                dtype: torch.dtype | None = None) -> torch.Tensor:
     """x [..., k] quantised along k, times w [n, k]: [..., n] in x's dtype unless another is given"""
-    flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    flat = x if x.dim() == 2 else x.reshape(x.shape[:-1].numel(), x.shape[-1])
     if flat.shape[1] != w.cols:
         raise ValueError(f"the summed axes differ: {tuple(x.shape)} and {w.shape}")
     if _turned(flat):

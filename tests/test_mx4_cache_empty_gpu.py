@@ -10,6 +10,16 @@ gpu = pytest.mark.gpu
 
 
 @gpu
+@pytest.mark.parametrize("lead", [(2, 3), (4,), (2, 0), (3, 2, 5)])
+def test_linear_without_columns(ops, lead):  # noqa: F811
+    """a sum of no terms: the bias, for any leading dimensions"""
+    w, bias = ops.mx4_quantize(torch.empty(7, 0, device="cuda")), torch.arange(7.0, device="cuda")
+    got = ops.mx4_linear(torch.empty(*lead, 0, device="cuda"), w, bias)
+    assert got.shape == (*lead, 7) and torch.equal(got, bias.expand(*lead, 7))
+    assert bool((ops.mx4_linear(torch.empty(*lead, 0, device="cuda"), w) == 0).all())
+
+
+@gpu
 @pytest.mark.parametrize("dtype", TYPES)
 def test_read_of_no_sequences(ops, dtype):  # noqa: F811
     """every token is outside cu: zeros, through the C entry as through the Python one, and nothing beside the rows"""
