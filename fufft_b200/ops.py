@@ -719,7 +719,9 @@ def cache_conv(cache: SeqCache, lengths: torch.Tensor, taps: torch.Tensor, gate:
     """newest output of a causal convolution per sequence, [batch, channels]:
     gate[b, c] * sum_j taps[j, c // (channels // heads)] * x[b, lengths[b] - 1 - j, c]
     over j < min(lengths[b], len(taps)); taps [n_taps, heads] float32 or
-    bfloat16, gate [batch, channels] of `dtype` or None"""
+    bfloat16, gate [batch, channels] of `dtype` or None.  The same call gives
+    the same bits; in long histories another sequence's length can move the
+    last of them (the work is dealt by the lengths of the whole batch)"""
     n, heads, taps_pitch = _rows(taps, "taps")
     if taps.dtype not in (torch.float32, torch.bfloat16):
         raise TypeError("taps must be float32 or bfloat16")

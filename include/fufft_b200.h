@@ -465,9 +465,12 @@ fufft_status fufft_mx4_linear(const void* x, fufft_dtype x_dtype, int64_t m, int
  *     heads divides channels; taps fp32 or bf16 with taps_stride between lags;
  *     gate (dtype of out, may be NULL); positions without a page count as
  *     zeros, a length of zero gives zero.  Sums are fp32, in an order that
- *     depends on the sizes alone.  workspace: fufft_cache_conv_workspace
- *     bytes, 16-byte aligned, not used by anything else until the call's work
- *     has finished. */
+ *     depends on the sizes and on lengths alone: the same call gives the same
+ *     bits.  Long histories are dealt to CTAs by the lengths of the whole
+ *     batch, so there another sequence's length can move the last bits of a
+ *     result.  At most 65535 sequences.  workspace:
+ *     fufft_cache_conv_workspace bytes, 16-byte aligned, not used by anything
+ *     else until the call's work has finished. */
 typedef enum fufft_cache_kind { FUFFT_CACHE_MX4 = 0, FUFFT_CACHE_MX8 = 1 } fufft_cache_kind;
 typedef struct fufft_cache {
    uint8_t* codes;
