@@ -30,6 +30,7 @@ from __future__ import annotations
 import ctypes as ct
 
 import torch
+from torch import _C
 
 from ._lib import (CACHE_MX4, CACHE_MX8, DTYPE_BF16, DTYPE_F16, DTYPE_F32, LAYOUT_NATURAL, LAYOUT_R8,
                    LAYOUT_R8_BPERM, LAYOUT_R16, LAYOUT_R16_BPERM, MID_CONJ_MULTIPLY, MID_MULTIPLY, MID_NONE,
@@ -418,14 +419,27 @@ def pipeline_v16_bfp(aq, a_scale, bq, b_scale, n):
 _DTYPES = {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}
 
 
-def _queue(*operands) -> int:
-    """the current stream of the current device, as _stream, without making a stream object; every operand of the call
-    (tensors, Mx4, SeqCache, None) has to be there, since only its address goes on"""
-    device = torch._C._cuda_getDevice()   # looked up here: a torch without CUDA has no such name, and still imports this
-    for t in operands:
-        if t is not None and t.get_device() != device:
-            raise ValueError(f"an operand is on cuda:{t.get_device()}, the current device is cuda:{device}")
-    return torch._C._cuda_getCurrentRawStream(device)
+def _queue(device: int, *others) -> int:
+    """the current stream of the current device, as _stream, without making a stream object; `device`, an operand's, and
+    the call's other operands (tensors, None) have to be there, since only their addresses go on"""
+    current = _C._cuda_getDevice()   # looked up here: a torch without CUDA has no such name, and still imports this
+    if device != current:
+        raise ValueError(f"an operand is on {_name(device)}, the current device is {_name(current)}")
+    for t in others:
+        if t is not None and t.get_device() != current:
+            raise ValueError(f"an operand is on {_name(t.get_device())}, the current device is {_name(current)}")
+    return _C._cuda_getCurrentRawStream(current)
+
+
+def _name(device: int) -> str:
+    return "the host" if device < 0 else f"cuda:{device}"
+
+
+def _at(t: torch.Tensor) -> int:
+    """address of a contiguous tensor whose device is checked by itself (_queue)"""
+    if not t.is_contiguous():
+        raise ValueError("tensor must be contiguous")
+    return t.data_ptr()
 
 
 def _dtype(t: torch.dtype) -> int:
@@ -451,7 +465,7 @@ def _rows(t: torch.Tensor, what: str) -> tuple[int, int, int]:
 def _i32(t: torch.Tensor, n: int, what: str):
     if t.dtype != torch.int32 or t.shape != (n,):
         raise ValueError(f"{what} must be int32 with {n} entries")
-    return _ptr(t)
+    return _at(t)
 
 
 def _result(out: torch.Tensor | None, like: torch.Tensor, rows: int, cols: int, dtype: torch.dtype) -> tuple[torch.Tensor, int]:
@@ -460,6 +474,8 @@ def _result(out: torch.Tensor | None, like: torch.Tensor, rows: int, cols: int, 
         return like.new_empty((rows, cols), dtype=dtype), cols
     if out.dtype != dtype or out.shape != (rows, cols):
         raise ValueError(f"out must be {dtype} {(rows, cols)}")
+    if out.get_device() != like.get_device():
+        raise ValueError(f"out is on {_name(out.get_device())}, the operands are on {_name(like.get_device())}")
     return out, _rows(out, "out")[2]
 
 
@@ -468,7 +484,7 @@ class Mx4:
     codes uint8 [rows, ceil(cols / 256) * 128] and the tiled E8M0 scales uint8
     [ceil(rows / 128), ceil(cols / 256) * 2, 32, 4, 4] (layout in
     include/fufft_b200.h, fufft_mx4_*)"""
-    __slots__ = ("_codes", "_scales", "_buffer", "_device", "rows", "cols", "at")
+    __slots__ = ("_codes", "_scales", "_buffer", "rows", "cols", "at", "device")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, cols: int):
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
@@ -477,14 +493,10 @@ class Mx4:
         if codes.numel() != rows * tiles * 64 or scales.numel() != -(-rows // 128) * tiles * 512:
             raise ValueError(f"codes or scales do not fit a {rows} x {cols} matrix")
         self._codes, self._scales, self._buffer, self.rows, self.cols = codes, scales, codes, rows, cols
-        self.at = _ptr(codes), _ptr(scales)
-        self._device = codes.get_device()
-        if scales.get_device() != self._device:
-            raise ValueError(f"codes are on cuda:{self._device}, scales on cuda:{scales.get_device()}")
-
-    def get_device(self) -> int:
-        """index of the device, as a tensor's"""
-        return self._device
+        self.at = _at(codes), _at(scales)
+        self.device = device = codes.get_device()
+        if device < 0 or scales.get_device() != device:
+            raise ValueError(f"codes and scales must be on one CUDA device, not {_name(device)} and {_name(scales.get_device())}")
 
     @property
     def codes(self) -> torch.Tensor:
@@ -513,7 +525,7 @@ def _mx4_new(like: torch.Tensor, rows: int, cols: int) -> Mx4:
     codes = rows * tiles * 64          # a multiple of 128
     q._buffer = like.new_empty(codes + -(-rows // 128) * tiles * 512, dtype=torch.uint8)
     q._codes = q._scales = None
-    q._device, q.rows, q.cols = q._buffer.get_device(), rows, cols
+    q.rows, q.cols, q.device = rows, cols, q._buffer.get_device()
     at = q._buffer.data_ptr()
     q.at = at, at + codes
     return q
@@ -542,7 +554,7 @@ def mx4_quantize(x: torch.Tensor, transpose: bool = False) -> Mx4:
     else:
         q = _mx4_new(x, rows, cols)
         at = *q.at, None, None
-    rc = lib().fufft_mx4_quantize(x.data_ptr(), dtype, rows, cols, pitch, *at, _queue(x))
+    rc = lib().fufft_mx4_quantize(x.data_ptr(), dtype, rows, cols, pitch, *at, _queue(x.get_device()))
     if rc:
         check(rc, "fufft_mx4_quantize")
     return q
@@ -555,7 +567,7 @@ def mx4_quantize_both(x: torch.Tensor) -> tuple[Mx4, Mx4]:
     rows, cols, pitch = _rows(x, "x")
     dtype = _dtype(x.dtype)
     q, qt = _mx4_new(x, rows, cols), _mx4_new(x, cols, rows)
-    rc = lib().fufft_mx4_quantize(x.data_ptr(), dtype, rows, cols, pitch, *q.at, *qt.at, _queue(x))
+    rc = lib().fufft_mx4_quantize(x.data_ptr(), dtype, rows, cols, pitch, *q.at, *qt.at, _queue(x.get_device()))
     if rc:
         check(rc, "fufft_mx4_quantize")
     return q, qt
@@ -565,7 +577,7 @@ def mx4_dequantize(q: Mx4, dtype: torch.dtype = torch.float32, out: torch.Tensor
     """the values that q stands for"""
     code = _dtype(dtype)
     out, pitch = _result(out, q._buffer, q.rows, q.cols, dtype)
-    rc = lib().fufft_mx4_dequantize(*q.at, q.rows, q.cols, out.data_ptr(), code, pitch, _queue(q, out))
+    rc = lib().fufft_mx4_dequantize(*q.at, q.rows, q.cols, out.data_ptr(), code, pitch, _queue(q.device))
     if rc:
         check(rc, "fufft_mx4_dequantize")
     return out
@@ -574,7 +586,7 @@ def mx4_dequantize(q: Mx4, dtype: torch.dtype = torch.float32, out: torch.Tensor
 def _bias(bias: torch.Tensor | None, n: int):
     if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,)):
         raise ValueError(f"bias must be float32 with {n} entries")
-    return _ptr(bias)
+    return None if bias is None else _at(bias)
 
 
 def mx4_matmul(a: Mx4, b: Mx4, dtype: torch.dtype = torch.bfloat16, bias: torch.Tensor | None = None,
@@ -583,10 +595,12 @@ def mx4_matmul(a: Mx4, b: Mx4, dtype: torch.dtype = torch.bfloat16, bias: torch.
     blocked along the summed axis, bias is float32 [b.rows]"""
     if a.cols != b.cols:
         raise ValueError(f"the summed axes differ: {a.shape} and {b.shape}")
+    if a.device != b.device:
+        raise ValueError(f"the operands are on {_name(a.device)} and {_name(b.device)}")
     code = _dtype(dtype)
     out, pitch = _result(out, a._buffer, a.rows, b.rows, dtype)
     rc = lib().fufft_mx4_matmul(*a.at, *b.at, _bias(bias, b.rows), out.data_ptr(), code, a.rows, b.rows, a.cols, pitch,
-                                _queue(a, b, bias, out))
+                                _queue(a.device, bias))
     if rc:
         check(rc, "fufft_mx4_matmul")
     return out
@@ -606,7 +620,7 @@ def mx4_linear(x: torch.Tensor, w: Mx4, bias: torch.Tensor | None = None,
     out = flat.new_empty((m, w.rows), dtype=dtype)
     q = None if m <= MX4_DIRECT_ROWS else _mx4_new(flat, m, k)   # few rows are quantised inside the product
     rc = lib().fufft_mx4_linear(flat.data_ptr(), codes, m, k, pitch, *(q.at if q else (None, None)), *w.at, w.rows,
-                                _bias(bias, w.rows), out.data_ptr(), out_code, w.rows, _queue(flat, w, bias))
+                                _bias(bias, w.rows), out.data_ptr(), out_code, w.rows, _queue(w.device, flat, bias))
     if rc:
         check(rc, "fufft_mx4_linear")
     return out if x.dim() == 2 else out.view(*x.shape[:-1], w.rows)
@@ -637,7 +651,7 @@ class SeqCache:
       codes       uint8 [pages, page_size, channels / 2 (mx4) or channels (mx8)]
       scales      uint8 [pages, page_size, channels / 32]
       page_table  int32 [batch, max_pages], -1 where there is no page"""
-    __slots__ = ("codes", "scales", "page_table", "kind", "channels", "batch", "desc", "at", "_device")
+    __slots__ = ("codes", "scales", "page_table", "kind", "channels", "batch", "desc", "at", "device")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, page_table: torch.Tensor, kind: str):
         code = _KINDS.get(kind)
@@ -653,17 +667,13 @@ class SeqCache:
             raise ValueError("codes and scales differ in their pages or channels")
         self.batch, max_pages, stride = _rows(page_table, "page_table")
         self.codes, self.scales, self.page_table, self.kind, self.channels = codes, scales, page_table, kind, channels
-        self.desc = CacheDesc(_ptr(codes), _ptr(scales), page_table.data_ptr(), stride, code, channels, page_size, pages,
+        self.desc = CacheDesc(_at(codes), _at(scales), page_table.data_ptr(), stride, code, channels, page_size, pages,
                               max_pages, self.batch)
         self.at = ct.addressof(self.desc)
-        self._device = codes.get_device()
-        if scales.get_device() != self._device or page_table.get_device() != self._device:
-            raise ValueError(f"codes are on cuda:{self._device}, scales on cuda:{scales.get_device()}, "
-                             f"page_table on cuda:{page_table.get_device()}")
-
-    def get_device(self) -> int:
-        """index of the device, as a tensor's"""
-        return self._device
+        self.device = device = codes.get_device()
+        if device < 0 or scales.get_device() != device or page_table.get_device() != device:
+            raise ValueError(f"codes, scales and page_table must be on one CUDA device, not {_name(device)}, "
+                             f"{_name(scales.get_device())} and {_name(page_table.get_device())}")
 
 
 def seq_cache(pages: int, page_size: int, channels: int, page_table: torch.Tensor, kind: str = "mx8") -> SeqCache:
@@ -682,7 +692,7 @@ def cache_append(cache: SeqCache, x: torch.Tensor, cu: torch.Tensor, starts: tor
     if channels != cache.channels:
         raise ValueError(f"x must have {cache.channels} channels")
     rc = lib().fufft_cache_append(cache.at, x.data_ptr(), _dtype(x.dtype), pitch, _i32(cu, cache.batch + 1, "cu"),
-                                  _i32(starts, cache.batch, "starts"), tokens, _queue(cache, x, cu, starts))
+                                  _i32(starts, cache.batch, "starts"), tokens, _queue(cache.device, x, cu, starts))
     if rc:
         check(rc, "fufft_cache_append")
 
@@ -693,7 +703,7 @@ def cache_read(cache: SeqCache, cu: torch.Tensor, starts: torch.Tensor, tokens: 
     code = _dtype(dtype)
     out, pitch = _result(out, cache.codes, tokens, cache.channels, dtype)
     rc = lib().fufft_cache_read(cache.at, out.data_ptr(), code, pitch, _i32(cu, cache.batch + 1, "cu"),
-                                _i32(starts, cache.batch, "starts"), tokens, _queue(cache, cu, starts, out))
+                                _i32(starts, cache.batch, "starts"), tokens, _queue(cache.device, cu, starts))
     if rc:
         check(rc, "fufft_cache_read")
     return out
@@ -707,7 +717,7 @@ def cache_read_channels(cache: SeqCache, starts: torch.Tensor, counts: torch.Ten
     code = _dtype(dtype)
     out = cache.codes.new_empty((cache.batch, cache.channels, n), dtype=dtype)
     rc = lib().fufft_cache_read_channels(cache.at, out.data_ptr(), code, n, _i32(starts, cache.batch, "starts"),
-                                         _i32(counts, cache.batch, "counts"), _queue(cache, starts, counts))
+                                         _i32(counts, cache.batch, "counts"), _queue(cache.device, starts, counts))
     if rc:
         check(rc, "fufft_cache_read_channels")
     return out
@@ -739,7 +749,7 @@ def cache_conv(cache: SeqCache, lengths: torch.Tensor, taps: torch.Tensor, gate:
     rc = lib().fufft_cache_conv(cache.at, _i32(lengths, cache.batch, "lengths"), taps.data_ptr(), _DTYPES[taps.dtype], n,
                                 heads, taps_pitch, gate_at, gate_pitch, out.data_ptr(), code, pitch, _ptr(workspace),
                                 0 if workspace is None else workspace.numel(),
-                                _queue(cache, lengths, taps, gate, out, workspace))
+                                _queue(cache.device, lengths, taps, gate, workspace))
     if rc:
         check(rc, "fufft_cache_conv")
     return out

@@ -102,9 +102,42 @@ def test_all_operands_elsewhere_are_refused(name):
         call()
 
 
-def test_matrices_of_another_device_are_refused_in_the_backward():
-    """the products that a backward pass makes of matrices kept from the forward"""
+@pytest.mark.parametrize("elsewhere", ["a", "b", "both"])
+def test_a_matrix_elsewhere_is_refused(elsewhere):
+    """whole matrices of another device, which their constructor has no reason to refuse"""
     here, there = _tensors(lambda k: Here), _tensors(lambda k: There)
-    a = ops.Mx4(here["a_codes"], here["a_scales"], 8, 64)
+    t = there if elsewhere in ("a", "both") else here
+    a = ops.Mx4(t["a_codes"], t["a_scales"], 8, 64)
+    t = there if elsewhere in ("b", "both") else here
+    b = ops.Mx4(t["codes"], t["scales"], 16, 64)
+    for out in (None, here["y"], there["y"]):
+        with pytest.raises(ValueError, match="cuda:1"):
+            ops.mx4_matmul(a, b, torch.float32, out=out)
+    if elsewhere != "a":
+        for x in (here["x"], here["x4"], there["x"], there["x4"]):
+            with pytest.raises(ValueError, match="cuda:1"):
+                ops.mx4_linear(x, b)
+    if elsewhere != "b":
+        for out in (None, here["wide"], there["wide"]):
+            with pytest.raises(ValueError, match="cuda:1"):
+                ops.mx4_dequantize(a, out=out)
+
+
+@pytest.mark.parametrize("name", ["append", "read", "read_channels", "conv"])
+def test_a_cache_elsewhere_is_refused(name):
+    t = {k: (There if k in ("cache_codes", "cache_scales", "table") else Here) for k in _tensors(lambda k: Here)}
+    call, _ = _calls(_tensors(t.get))[name]
     with pytest.raises(ValueError, match="cuda:1"):
-        ops.mx4_matmul(a, ops.Mx4(there["codes"], there["scales"], 16, 64))
+        call()
+
+
+def test_tensors_of_the_host_are_refused():
+    t = _tensors(lambda k: torch.Tensor)
+    for call, operands in _calls(t).values():
+        with pytest.raises(ValueError):
+            call()
+    for name, (_, operands) in _calls(_tensors(lambda k: Here)).items():
+        for operand in operands:
+            call, _ = _calls(_tensors(lambda k: torch.Tensor if k == operand else Here))[name]
+            with pytest.raises(ValueError):
+                call()
