@@ -15,7 +15,7 @@ namespace fufft {
 namespace cache {
 
 constexpr int CH = 16;        // channels per thread: one 8-byte (MX4) or 16-byte (MX8) load a token
-constexpr int TILE = 1024;    // lags whose cache rows are looked up together, at most (1 x 16384 x 32 MX4: 9.0 us, with 256 10.3)
+constexpr int TILE = 1024;    // lags whose cache rows are looked up together, at most (1 x 16384 x 32 MX4: 8.8 us, with 256 10.3)
 constexpr int THREADS = 256;
 constexpr int MAX_SPLIT = 8;    // CTAs of a portable cluster
 
@@ -179,8 +179,9 @@ __device__ __forceinline__ void join(float* joined, const ConvStep& a, const Pag
 // a stored value is a number of 32 bits, exactly, where a scale of 2^124 times
 // a tap need not be.  One exact fma widens and scales it where the scale is a
 // half-precision number, two operations where a scale of the thread's batch is
-// not (5 x 5000 x 2112 MX4, 22 heads: 12.7 us, 14.8 if all took two); half a
-// packed fma adds it times its tap.
+// not (5 x 5000 x 2112 MX4, 3001 taps of 22 heads: 12.7 us, 14.8 if all took
+// two); half a packed fma adds it times its tap.  The variants whose taps are
+// gathered spill, up to 250 bytes with four sequences and fp32 taps.
 // CTAs of a cluster take tiles of lags in turn and join through distributed
 // shared memory, in rank order.
 template<bool MX8, class TT, Taps MODE, int NB>
@@ -304,9 +305,10 @@ __global__ void __launch_bounds__(256) conv_join_kernel(ConvStep a, int batch)
 // 29 values a clock and SM, 49 this way).  Where rows are missing, each row is
 // asked for first (16 sequences of 16384 to 32768, one empty, x 2048 MX4: 171
 // us; 201 where such stages took the general way).
-// 16 x 32768 x 2048 MX4, bf16 taps: 200 us, floor 107; the sums alone, without
-// a ring to wait for, 165 (130 with taps that heads share, which are read and
-// widened once a block).  Sixteen warps of eight channels a thread: the sums
+// 16 x 32768 x 2048 MX4, bf16 taps: 199 us, floor 107 (a scale of zero in one
+// token of 64 takes every stage the general way: 228); taps that heads share
+// 208, MX8 259.  The sums alone, without a ring to wait for, 165 (130 with taps
+// that heads share, which are read and widened once a block).  Sixteen warps of eight channels a thread: the sums
 // alone 171, with the ring 212.
 // ---------------------------------------------------------------------------
 namespace pipe {
@@ -805,8 +807,9 @@ bool plan(long long lags, bool mx8, int channels, int batch, int tap_size, int s
    // share for each group 194 us, dealt 73).
    const double value = mx8 ? 33.0 / 32 : 17.0 / 32;
    const bool small = (double)lags * channels * (batch * value + tap_size) < 64.0 * (1 << 20);
-   // scales that have to be read byte by byte are worth it for long histories only (5 x 5000 x 2112 MX4: 105 us, 65
-   // without the ring)
+   // scales that have to be read byte by byte are worth it for long histories only (us, ring / direct: 5 ragged to
+   // 5000 x 2112 MX4, 3001 taps of 22 heads 53.2 / 13.0; 1 x 5000 x 2112, a filter a channel 16.4 / 12.1; 4 x 2000 x 1088 MX8
+   // 23.0 / 16.4)
    if(small && channels % 128) return false;
    const auto lay = [&](int chunks) {
       p->lanes = (int)mx::ceil_div(mx::ceil_div(units, chunks), grain) * grain;

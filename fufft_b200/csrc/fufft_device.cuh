@@ -235,8 +235,9 @@ __device__ __forceinline__ void prefetch_l2_bulk(const void* src, uint32_t bytes
    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" :: "l"(src), "r"(bytes) : "memory");
 }
 // 2-D tiled TMA load of box (x, y) of a tensor map into shared memory,
-// completion on `bar`.  Every CTA loads its own tiles from this GPU's memory.  x is
-// always 0 here (whole 128-byte rows), so the 16-byte rule on x holds.
+// completion on `bar`.  Every CTA loads its own tiles from this GPU's memory.  x
+// times the element size is a multiple of 16 bytes (callers step by whole
+// 128-byte rows).
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* tm, int x, int y, uint64_t* bar)
 {
    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"

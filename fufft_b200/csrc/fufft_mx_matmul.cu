@@ -661,7 +661,8 @@ template<class T> fufft_status matmul(const Operands& o, cudaStream_t st)
    if(chunks == 0) return launch_split<T, 128>(o, 1, ctx, st);
    // 256 columns in one accumulator or 192 in two of them, whichever covers the
    // result in fewer columns' time (us, 256 / 192: 8192^3 189 / 201, 4096^3
-   // 28.1 / 26.7, 512 x 4096 x 4096 10.3 / 9.0)
+   // 28.1 / 26.7, 512 x 4096 x 4096 10.3 / 9.0).  The drain after a tile's
+   // last stage, which a single accumulator cannot hide, is not in the rule.
    return ceil_div(wide, pairs) * 256 < ceil_div(narrow, pairs) * 192 ? launch_pair<T, Pair<256, 1>>(o, ctx, st)
                                                                      : launch_pair<T, Pair<192, 2>>(o, ctx, st);
 }

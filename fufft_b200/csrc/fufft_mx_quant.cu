@@ -43,7 +43,8 @@ template<class T> bool rows_on_32(const void* p, long long row_stride)
 // Rows: a warp takes U x 512 columns of a row, a lane sixteen of each, two
 // lanes a block, eight lanes the four blocks of a scale word.  Columns beyond
 // `cols` are zeros.  Bound by reading x and writing the codes (16384^2 bf16 98
-// us, floor 104; 8192^2 fp32 46).
+// us; its bytes at the rate of a plain copy, half of which are writes, 104;
+// 8192^2 bf16 27, fp32 46).
 constexpr int SPAN = 32 * HALF;   // columns of a warp's pass
 constexpr int STAGE = SPAN + SPAN / HALF;
 
